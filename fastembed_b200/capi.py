@@ -97,6 +97,14 @@ _SIGS = {
     "fe_token_positions": ([vp, i32, vp, vp], C.c_int),
     "fe_qk_norm_rope_bf16": ([vp, vp, i32, i64, i32, i32, i32, vp, vp, i32, f32, f32, vp], C.c_int),
     "fe_pool_l2": ([vp, vp, i32, i32, C.c_int, vp, vp], C.c_int),
+    "fe_quantize_rows_e4m3": ([vp, C.c_int, i64, i32, vp, vp, vp], C.c_int),
+    "fe_add_rmsnorm_e4m3": ([vp, C.c_int, vp, vp, i32, f32, i64, i32, vp, vp, vp], C.c_int),
+    "fe_linear_e4m3": ([vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, C.c_int, vp], C.c_int),
+    "fe_kv_cache_append_e4m3": ([vp, vp, i32, i32, i64, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, vp],
+                                C.c_int),
+    "fe_attention_cache_workspace_bytes": ([i32, i32, i64, i32, i32, i32, i32, C.POINTER(sz)], C.c_int),
+    "fe_attention_cache_e4m3": ([vp, vp, i32, i32, i64, i32, i32, i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32,
+                                 f32, vp, vp, sz, vp], C.c_int),
     "fe_engine_create": ([C.POINTER(EncoderConfig), C.c_int, C.POINTER(vp)], C.c_int),
     "fe_engine_create_rms": ([C.POINTER(RmsEncoderConfig), C.c_int, C.POINTER(vp)], C.c_int),
     "fe_engine_destroy": ([vp], C.c_int),

@@ -48,6 +48,7 @@ uint64_t current_context_id();
 cudaError_t set_wait_limit_linear(uint64_t ns);
 cudaError_t set_wait_limit_attention(uint64_t ns);
 cudaError_t set_wait_limit_attention_wide(uint64_t ns);
+cudaError_t set_wait_limit_linear_e4m3(uint64_t ns);
 int current_sm_count();
 // Programmatic dependent launch for the kernels that call grid_dep_wait(): on with
 // FE_PDL=1 (read once per process), off by default.  On bge-large, Qwen3- and
@@ -150,6 +151,28 @@ cudaError_t launch_layernorm_dual_bf16in(const void *x, const float *res, const 
 cudaError_t launch_pool_l2(const float *h, const int32_t *cu, int batch, int dim, int mode,
                            float *out, cudaStream_t s);
 cudaError_t launch_f32_to_bf16(const float *x, void *y, int64_t count, cudaStream_t s);
+
+// ---- 8-bit (e4m3) operators ----
+cudaError_t launch_quantize_rows_e4m3(const void *x, int x_dtype, int64_t rows, int dim, void *q, float *scale,
+                                      cudaStream_t s);
+// h32 += y (y may be null), then the codes and scales of RMSNorm(h32) * (w, or 1 + w)
+cudaError_t launch_add_rmsnorm_e4m3(const void *y, int y_dtype, float *h32, const float *w, bool one_plus, float eps,
+                                    int64_t rows, int dim, void *q, float *scale, cudaStream_t s);
+cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, const float *sw, const float *bias,
+                               const float *residual, void *y, int64_t m, int64_t n, int64_t k, int epilogue, int y_dtype,
+                               cudaStream_t s, fe_status *st);
+// head_dim 64 / 128 / 256, page 16 / 32 / 64 / 128
+cudaError_t launch_kv_cache_append_e4m3(const void *qkv, const int32_t *cu, int batch, int max_len, int64_t total,
+                                        int q_heads, int kv_heads, int head_dim, const int32_t *past, const int32_t *table,
+                                        int width, void *k, void *v, float *ks, float *vs, int pages, int page,
+                                        cudaStream_t s);
+size_t attention_cache_workspace_bytes(int batch, int max_len, int64_t total, int max_kv, int q_heads, int kv_heads,
+                                       int head_dim);
+cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int batch, int max_len, int64_t total,
+                                        int q_heads, int kv_heads, int head_dim, const int32_t *past, int max_kv,
+                                        const int32_t *table, int width, const void *k, const void *v, const float *ks,
+                                        const float *vs, int pages, int page, bool causal, float scale, void *out,
+                                        void *workspace, cudaStream_t s);
 
 cudaError_t launch_sgemm(const float *a, const float *b, const float *bias, float *c, int64_t m,
                          int64_t n, int64_t k, bool b_transposed, cudaStream_t s);

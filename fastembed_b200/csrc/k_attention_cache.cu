@@ -1,0 +1,555 @@
+// k_attention_cache.cu — attention of new tokens over the paged 8-bit key-value cache.
+//
+//     out_i = sum_j p_ij v_j,   p_ij = softmax_j(scale * q_i . k_j),   j <= past + i (causal)
+//                                                                  or j < past + len
+// with k_j = kc_j sk(page), v_j = vc_j sv(page): e4m3 codes times the scale of their page and
+// head.  The scales leave the products:
+//     s_ij = (scale log2 e) sk q_i . kc_j          (base-2 logits)
+//     t_ij = s_ij + log2 sv,   P_ij = 2^(t_ij - m_i),   m_i = max_j t_ij - 15
+//     out_i = (sum_j P_ij vc_j) / (sum_j 2^(s_ij - m_i))
+// so the value scale moves into the exponent, the running maximum is that of the weights as they
+// meet the codes, and P (at most 2^15) keeps 11 bits in f16 with nothing above 2^-39 of the
+// largest weight lost, whatever the pages' scales are.  Statistics and sums are fp32.
+//
+// attn_cache_stream: the form for few rows (single tokens).  A key-value head's rows are its
+// query heads' new tokens together, r = token * group + head, 8 NR of them to a CTA.  Nothing is
+// shared between warps but the final sum: each warp takes every WARPS-th run of 32 tokens of its
+// CTA's part of the sequence and streams the codes from global memory straight into the
+// fragments of mma.m16n8k16, no shared memory in between.
+//   S^T [tokens x rows] = K Q^T: A is K.  A thread's 16 consecutive bytes of a token (one load)
+//     are the four k-pairs of four k-steps: the order of k inside the sum is free, so Q's
+//     fragments are loaded in that order once.
+//   O^T [hd x rows] = V^T P^T: A is V^T.  A thread reads 16 consecutive codes of four tokens and
+//     pairs them up by byte permutes; which hd row a fragment row stands for is free too (row g
+//     of m-tile i is hd 16 g + 2 i).  P^T in B-fragment form is the 8x8 transpose of S^T's
+//     accumulator.
+// Each e4m3 pair becomes f16x2 in one conversion (exact).  The sequence is split over CTAs when
+// there are too few to fill the GPU; attn_cache_join sums the parts.
+//
+// Pages beyond the sequence are never read; slots past its end are masked before they are used
+// (values zeroed: a slot never written may hold any code).  A page id outside the pool sets
+// FE_ERR_INVALID_ARGUMENT in the device status word and its tokens are left out.
+#include <algorithm>
+
+#include "fe_e4m3.cuh"
+#include "fe_internal.h"
+
+namespace fe {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBoost = 15.f;  // P is at most 2^15
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// D += A B, m16n8k16, f16 inputs, fp32 accumulator
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
+{
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ uint4 ld_stream16(const uint8_t *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ uint2 ld_stream8(const uint8_t *p)
+{
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+struct CacheArgs {
+    const __nv_bfloat16 *qkv;
+    const int32_t *cu, *past, *table;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    __nv_bfloat16 *out;
+    float *part_o;  // [T * q_heads][splits][hd], splits > 1
+    float *part_ml; // [T * q_heads][splits][2]: m, l
+    int64_t total, row;
+    int batch, max_len, width, pages, page_log2, q_heads, kv_heads, group, causal;
+    int splits;
+    float scale_log2;
+};
+
+// One sequence of the batch: false (and a report) when its offsets do not describe it.
+struct Seq {
+    int t0, len, past, kv;  // first row, new tokens, tokens before them, tokens in the cache
+};
+__device__ __forceinline__ bool load_seq(const CacheArgs &a, int b, Seq &s, int *status)
+{
+    s.t0 = a.cu[b];
+    const int t1 = a.cu[b + 1];
+    s.past = a.past[b];
+    s.len = t1 - s.t0;
+    if (s.len <= 0) return false;
+    const int64_t kv = static_cast<int64_t>(s.past) + s.len;
+    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 && kv <= (static_cast<int64_t>(a.width) << a.page_log2);
+    s.kv = static_cast<int>(kv);
+    if (!ok && threadIdx.x == 0) report(status, DEV_BAD_INPUT);
+    return ok;
+}
+
+constexpr int kWarpTokens = 32;
+
+template <int HD, int NR, int WARPS>
+struct StreamCfg {
+    static constexpr int ROWS = 8 * NR;
+    static constexpr int LD = HD + 4;  // floats per row of the joining buffer
+    static constexpr uint32_t SMEM = WARPS * ROWS * (LD + 2) * 4;
+};
+
+template <int HD, int NR, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs a, int row_tiles, int *status)
+{
+    using C = StreamCfg<HD, NR, WARPS>;
+    constexpr int KC = HD / 64;            // 16-byte chunks of a token's key per thread
+    constexpr int VB = HD >= 128 ? 16 : 8; // bytes of a token's value per thread and 128 (64) codes
+    constexpr int VC = HD >= 128 ? HD / 128 : 1;
+    constexpr int VW = VB / 4;             // words of those
+    constexpr int MT = HD / 16;            // m-tiles of O^T
+    extern __shared__ float join[];        // [WARPS][ROWS][LD], then [WARPS][ROWS][2]
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, c = lane & 3;
+    const int split = blockIdx.z, kvh = blockIdx.y;
+    const int b = blockIdx.x / row_tiles, tile = blockIdx.x % row_tiles;
+    grid_dep_wait();
+    grid_dep_launch();
+    Seq sq;
+    if (!load_seq(a, b, sq, status)) return;
+    const int rows = sq.len * a.group, r0 = tile * C::ROWS;
+    if (r0 >= rows) return;
+
+    // Q fragments (column n = g of each 8-row tile), each row brought to [1, 2) at its maximum by
+    // a power of two so that f16 holds every bf16 of it
+    uint32_t qf[NR][KC][4][2];
+    float qs[NR][2];   // base-2 logit factor of rows 2c, 2c + 1
+    int lim[NR][2];    // last visible token of rows 2c, 2c + 1 (-1: no such row)
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int r = r0 + 8 * n + g;
+        float f[KC][16];
+        float m = 0.f;
+        if (r < rows) {
+            const __nv_bfloat16 *p =
+                a.qkv + (sq.t0 + r / a.group) * a.row + static_cast<int64_t>(kvh * a.group + r % a.group) * HD + 16 * c;
+#pragma unroll
+            for (int j = 0; j < KC; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(p + 64 * j + 8 * h);
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 x = unpack_bf16x2(w[i]);
+                        f[j][8 * h + 2 * i] = x.x;
+                        f[j][8 * h + 2 * i + 1] = x.y;
+                        m = fmaxf(m, fmaxf(finite_abs(x.x), finite_abs(x.y)));
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < KC; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) f[j][i] = 0.f;
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // 2^-e and 2^e of the row's exponent, e in [-100, 127]
+        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+        e = e < -100 ? -100 : e;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + (e > 126 ? 126 : e)) << 23);
+#pragma unroll
+        for (int j = 0; j < KC; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                qf[n][j][q][0] = pack_f16x2(f[j][4 * q] * down, f[j][4 * q + 1] * down);
+                qf[n][j][q][1] = pack_f16x2(f[j][4 * q + 2] * down, f[j][4 * q + 3] * down);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int rr = r0 + 8 * n + 2 * c + h;
+            qs[n][h] = __shfl_sync(0xffffffffu, up, (2 * c + h) * 4) * a.scale_log2;
+            lim[n][h] = rr >= rows ? -1 : a.causal ? sq.past + rr / a.group : sq.kv - 1;
+        }
+    }
+    // tokens this CTA reads: its part of those its last row sees
+    const int last_row = min(r0 + C::ROWS, rows) - 1;
+    const int end_all = a.causal ? sq.past + last_row / a.group + 1 : sq.kv;
+    const int runs = (end_all + kWarpTokens - 1) / kWarpTokens;
+    const int per = (runs + a.splits - 1) / a.splits;
+    const int run0 = split * per, run1 = min(run0 + per, runs);
+
+    float o[NR][MT][4];
+    float mx[NR][2], l[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
+        mx[n][0] = mx[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+    }
+
+    const int32_t *tab = a.table + static_cast<int64_t>(b) * a.width;
+    const int page_mask = (1 << a.page_log2) - 1;
+    for (int run = run0 + warp; run < run1; run += WARPS) {
+        // 32 tokens = two 16-token tiles, each inside one page (pages are 16 tokens or more)
+        uint4 kf[2][2][KC];          // [tile][token g / g + 8][chunk]
+        uint32_t vf[2][4][VC][VW];   // [tile][token 2c, 2c + 1, 2c + 8, 2c + 9][chunk][word]
+        float sk[2], sv[2];
+        bool have[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int tok = run * kWarpTokens + 16 * u;
+            int id = -1;
+            if (tok < end_all) {
+                id = __ldg(tab + (tok >> a.page_log2));
+                if (id < 0 || id >= a.pages) {
+                    if (lane == 0) report(status, DEV_BAD_INPUT);
+                    id = -1;
+                }
+            }
+            have[u] = id >= 0;
+            if (have[u]) {
+                const int64_t ph = static_cast<int64_t>(id) * a.kv_heads + kvh;
+                const int64_t at = ((ph << a.page_log2) + (tok & page_mask)) * HD;
+                const uint8_t *kp = a.k + at + g * HD + 16 * c, *vp = a.v + at + 2 * c * HD + VB * g;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+                    kf[u][0][j] = ld_stream16(kp + 64 * j);
+                    kf[u][1][j] = ld_stream16(kp + 8 * HD + 64 * j);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VC; ++j) {
+                        const uint8_t *p = vp + ((i & 1) + 8 * (i >> 1)) * HD + 128 * j;
+                        if constexpr (VB == 16) {
+                            const uint4 x = ld_stream16(p);
+                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y, vf[u][i][j][2] = x.z, vf[u][i][j][3] = x.w;
+                        } else {
+                            const uint2 x = ld_stream8(p);
+                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y;
+                        }
+                    }
+                sk[u] = __ldg(a.ks + ph);
+                sv[u] = __ldg(a.vs + ph);
+            } else {
+                sk[u] = sv[u] = 0.f;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) kf[u][0][j] = kf[u][1][j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VC; ++j)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vf[u][i][j][w] = 0;
+            }
+        }
+        // S^T: accumulator (token g, row 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1)
+        float s[NR][2][4];
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][u][i] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < KC; ++j) {
+                const uint32_t lo[4] = {kf[u][0][j].x, kf[u][0][j].y, kf[u][0][j].z, kf[u][0][j].w};
+                const uint32_t hi[4] = {kf[u][1][j].x, kf[u][1][j].y, kf[u][1][j].z, kf[u][1][j].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t a0 = e4m3x2_to_f16x2(lo[q]), a1 = e4m3x2_to_f16x2(hi[q]);
+                    const uint32_t a2 = e4m3x2_to_f16x2(lo[q] >> 16), a3 = e4m3x2_to_f16x2(hi[q] >> 16);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) mma_f16(s[n][u], a0, a1, a2, a3, qf[n][j][q][0], qf[n][j][q][1]);
+                }
+            }
+        // base-2 logits, masked; t = s + log2 sv (a page of zero values adds nothing: log2 -> 0)
+        float ev[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) ev[u] = sv[u] > 0.f ? log2f(sv[u]) : 0.f;
+        uint32_t pt[NR][2][2];  // P^T fragments [tile][tokens 2c.. / 2c + 8..]
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            float top[2] = {mx[n][0], mx[n][1]};
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = run * kWarpTokens + 16 * u + g + 8 * (i >> 1);
+                    const bool on = have[u] && tok <= lim[n][i & 1];
+                    s[n][u][i] = on ? s[n][u][i] * (sk[u] * qs[n][i & 1]) : -INFINITY;
+                    top[i & 1] = fmaxf(top[i & 1], s[n][u][i] + ev[u]);
+                }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+            }
+            const bool grew = top[0] > mx[n][0] || top[1] > mx[n][1];
+            if (__any_sync(0xffffffffu, grew)) {
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f[h] = mx[n][h] == -INFINITY ? 0.f : exp2_fast(mx[n][h] - top[h]);
+                    mx[n][h] = top[h];
+                    l[n][h] *= f[h];
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    o[n][i][0] *= f[0];
+                    o[n][i][1] *= f[1];
+                    o[n][i][2] *= f[0];
+                    o[n][i][3] *= f[1];
+                }
+            }
+            const float ref[2] = {mx[n][0] == -INFINITY ? 0.f : mx[n][0] - kBoost,
+                                  mx[n][1] == -INFINITY ? 0.f : mx[n][1] - kBoost};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[i] = exp2_fast(s[n][u][i] + ev[u] - ref[i & 1]);
+                    l[n][i & 1] += exp2_fast(s[n][u][i] - ref[i & 1]);
+                }
+                pt[n][u][0] = transpose8x8(pack_f16x2(p[0], p[1]));
+                pt[n][u][1] = transpose8x8(pack_f16x2(p[2], p[3]));
+            }
+        }
+        // slots past the sequence's end hold anything, a NaN code among it: 0 * NaN would be NaN
+        if (run * kWarpTokens + kWarpTokens > sq.kv) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (run * kWarpTokens + 16 * u + 2 * c + (i & 1) + 8 * (i >> 1) >= sq.kv) {
+#pragma unroll
+                        for (int j = 0; j < VC; ++j)
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) vf[u][i][j][w] = 0;
+                    }
+        }
+        // O^T: m-tile (j, 2 w) holds codes 4 w, 4 w + 1 of a thread's run, (j, 2 w + 1) the next two
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < VC; ++j)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    const uint32_t x0 = __byte_perm(vf[u][0][j][w], vf[u][1][j][w], 0x5140);
+                    const uint32_t x1 = __byte_perm(vf[u][0][j][w], vf[u][1][j][w], 0x7362);
+                    const uint32_t y0 = __byte_perm(vf[u][2][j][w], vf[u][3][j][w], 0x5140);
+                    const uint32_t y1 = __byte_perm(vf[u][2][j][w], vf[u][3][j][w], 0x7362);
+                    const uint32_t a0 = e4m3x2_to_f16x2(x0), a1 = e4m3x2_to_f16x2(x0 >> 16);
+                    const uint32_t a2 = e4m3x2_to_f16x2(y0), a3 = e4m3x2_to_f16x2(y0 >> 16);
+                    const uint32_t b0 = e4m3x2_to_f16x2(x1), b1 = e4m3x2_to_f16x2(x1 >> 16);
+                    const uint32_t b2 = e4m3x2_to_f16x2(y1), b3 = e4m3x2_to_f16x2(y1 >> 16);
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) {
+                        mma_f16(o[n][2 * VW * j + 2 * w], a0, a1, a2, a3, pt[n][u][0], pt[n][u][1]);
+                        mma_f16(o[n][2 * VW * j + 2 * w + 1], b0, b1, b2, b3, pt[n][u][0], pt[n][u][1]);
+                    }
+                }
+    }
+
+    // join the warps: each leaves its rows' m, l and O, then the CTA sums them
+    float *ml = join + WARPS * C::ROWS * C::LD;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float t = l[n][h];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+            const int r = 8 * n + 2 * c + h;
+            if (g == 0) {
+                ml[(warp * C::ROWS + r) * 2] = mx[n][h];
+                ml[(warp * C::ROWS + r) * 2 + 1] = t;
+            }
+            float *dst = join + (warp * C::ROWS + r) * C::LD;
+#pragma unroll
+            for (int j = 0; j < VC; ++j)
+#pragma unroll
+                for (int i = 0; i < 2 * VW; ++i) {
+                    const int mt = 2 * VW * j + i, hd = 128 * j + VB * g + 2 * i;
+                    *reinterpret_cast<float2 *>(dst + hd) = make_float2(o[n][mt][h], o[n][mt][2 + h]);
+                }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < C::ROWS * HD / 4; i += 32 * WARPS) {
+        const int r = i / (HD / 4), hd = i % (HD / 4) * 4;
+        if (r0 + r >= rows) break;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[(w * C::ROWS + r) * 2]);
+        float sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float wm = ml[(w * C::ROWS + r) * 2];
+            const float f = wm == -INFINITY ? 0.f : exp2_fast(wm - m);
+            const float wl = ml[(w * C::ROWS + r) * 2 + 1];
+            const float4 x = *reinterpret_cast<const float4 *>(join + (w * C::ROWS + r) * C::LD + hd);
+            if (wm != -INFINITY || wl != 0.f) {  // NaN logits leave m behind: l carries them
+                const float k = wm == -INFINITY ? 1.f : f;
+                sum += wl * k;
+                acc.x += x.x * k, acc.y += x.y * k, acc.z += x.z * k, acc.w += x.w * k;
+            }
+        }
+        const int64_t orow = (sq.t0 + (r0 + r) / a.group) * static_cast<int64_t>(a.q_heads) + kvh * a.group + (r0 + r) % a.group;
+        if (a.splits == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a row that sees nothing is zero
+            *reinterpret_cast<uint2 *>(a.out + orow * HD + hd) =
+                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        } else {
+            const int64_t at = orow * a.splits + split;
+            *reinterpret_cast<float4 *>(a.part_o + at * HD + hd) = acc;
+            if (hd == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, sum);
+        }
+    }
+}
+
+// Sums the parts of each (token, query head) row of a sequence: a warp a row.
+template <int HD>
+__global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *status)
+{
+    const int lane = threadIdx.x & 31;
+    grid_dep_wait();
+    grid_dep_launch();
+    Seq sq;
+    if (!load_seq(a, blockIdx.y, sq, status)) return;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (i >= static_cast<int64_t>(sq.len) * a.q_heads) return;
+    const int64_t r = static_cast<int64_t>(sq.t0) * a.q_heads + i;
+    constexpr int V = HD / 32;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(r * a.splits + s) * 2]);
+    float sum = 0.f, acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r * a.splits + s) * 2);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
+        const float k = ml.x == -INFINITY ? 1.f : exp2_fast(ml.x - m);
+        sum += ml.y * k;
+        const float *p = a.part_o + (r * a.splits + s) * HD + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += p[i] * k;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    __nv_bfloat16 *dst = a.out + r * HD + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+}
+
+constexpr int kWarps = 4;
+
+// 8-row tiles of a CTA: 16 rows where the registers allow it and there are more than 8
+int row_tile_count(int rows, int head_dim) { return rows > 8 && head_dim < 256 ? 2 : 1; }
+
+template <int HD, int NR>
+cudaError_t stream(const CacheArgs &a, int *status, cudaStream_t s)
+{
+    using C = StreamCfg<HD, NR, kWarps>;
+    static_assert(C::SMEM <= 48 * 1024, "no opt-in shared memory");
+    const int row_tiles = (a.max_len * a.group + C::ROWS - 1) / C::ROWS;
+    cudaError_t e = launch_k(attn_cache_stream<HD, NR, kWarps>,
+                             dim3(static_cast<unsigned>(a.batch) * row_tiles, a.kv_heads, a.splits), dim3(32 * kWarps),
+                             C::SMEM, s, a, row_tiles, status);
+    if (e != cudaSuccess || a.splits == 1) return e;
+    return launch_k(attn_cache_join<HD>, dim3((static_cast<unsigned>(a.max_len) * a.q_heads + 3) / 4, a.batch), dim3(128), 0,
+                    s, a, status);
+}
+
+template <int HD>
+cudaError_t stream_any(const CacheArgs &a, int *status, cudaStream_t s)
+{
+    if constexpr (HD < 256)
+        if (row_tile_count(a.max_len * a.group, HD) == 2) return stream<HD, 2>(a, status, s);
+    return stream<HD, 1>(a, status, s);
+}
+
+}  // namespace
+
+// Parts the sequences are split into: enough CTAs for about four rounds of the resident ones
+// (sequences differ in length), each with 512 tokens or more of the longest.
+int attention_cache_splits(int batch, int max_len, int max_kv, int q_heads, int kv_heads, int head_dim)
+{
+    const int64_t rows = static_cast<int64_t>(max_len) * (q_heads / kv_heads);
+    const int per = 8 * row_tile_count(static_cast<int>(std::min<int64_t>(rows, 1 << 20)), head_dim);
+    const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
+    const int64_t want = (12ll * current_sm_count() + ctas - 1) / ctas;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+}
+
+size_t attention_cache_workspace_bytes(int batch, int max_len, int64_t total, int max_kv, int q_heads, int kv_heads,
+                                       int head_dim)
+{
+    const int64_t splits = attention_cache_splits(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    return splits == 1 ? 0 : static_cast<size_t>(total) * q_heads * splits * (head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int batch, int max_len, int64_t total,
+                                        int q_heads, int kv_heads, int head_dim, const int32_t *past, int max_kv,
+                                        const int32_t *table, int width, const void *k, const void *v, const float *ks,
+                                        const float *vs, int pages, int page, bool causal, float scale, void *out,
+                                        void *workspace, cudaStream_t s)
+{
+    CacheArgs a;
+    a.qkv = static_cast<const __nv_bfloat16 *>(qkv);
+    a.cu = cu, a.past = past, a.table = table;
+    a.k = static_cast<const uint8_t *>(k), a.v = static_cast<const uint8_t *>(v);
+    a.ks = ks, a.vs = vs;
+    a.out = static_cast<__nv_bfloat16 *>(out);
+    a.total = total;
+    a.row = static_cast<int64_t>(q_heads + 2 * kv_heads) * head_dim;
+    a.batch = batch, a.max_len = max_len, a.width = width, a.pages = pages;
+    a.page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+    a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.causal = causal;
+    a.scale_log2 = scale * kLog2e;
+    a.splits = attention_cache_splits(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = a.part_o + total * q_heads * a.splits * head_dim;
+    int *status = current_device_status_word();
+    if (head_dim == 64) return stream_any<64>(a, status, s);
+    if (head_dim == 128) return stream_any<128>(a, status, s);
+    return stream_any<256>(a, status, s);
+}
+
+}  // namespace fe

@@ -222,6 +222,7 @@ fe_status fe_set_wait_limit(int device, uint64_t limit_ns)
     if (e == cudaSuccess) e = fe::set_wait_limit_linear(limit_ns);
     if (e == cudaSuccess) e = fe::set_wait_limit_attention(limit_ns);
     if (e == cudaSuccess) e = fe::set_wait_limit_attention_wide(limit_ns);
+    if (e == cudaSuccess) e = fe::set_wait_limit_linear_e4m3(limit_ns);
     cudaSetDevice(prev);
     return fe::check_cuda(e, "fe_set_wait_limit");
 }
@@ -241,7 +242,7 @@ fe_status fe_device_status(int device)
     if (e != cudaSuccess) return fe::check_cuda(e, "fe_device_status");
     if (v == fe::DEV_TIMEOUT) return fe::fail(FE_ERR_DEVICE_TIMEOUT, "a kernel's bounded wait ran out");
     if (v == fe::DEV_BAD_INPUT)
-        return fe::fail(FE_ERR_INVALID_ARGUMENT, "a kernel met an out-of-range token id or position");
+        return fe::fail(FE_ERR_INVALID_ARGUMENT, "a kernel met an out-of-range token id, position, offset or page id");
     return FE_OK;
 }
 

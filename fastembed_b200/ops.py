@@ -4,6 +4,7 @@ FeError on a non-OK status.  PyTorch only supplies device memory and streams."""
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -278,6 +279,161 @@ def pool_l2(h, cu_seqlens, mode="cls"):
     D = h.shape[1]
     out = torch.empty(B, D, dtype=torch.float32, device=h.device)
     call("fe_pool_l2", _p(h), _p(cu_seqlens), B, D, POOL[mode], _p(out), _s(h))
+    return out
+
+
+# ------------------------------------------------------- 8-bit (e4m3) operators
+F8 = torch.float8_e4m3fn
+
+
+class KvCacheE4m3(NamedTuple):
+    """A paged 8-bit key-value cache: codes [pages, kv_heads, page_size, head_dim] and one fp32
+    scale per page and head [pages, kv_heads], for keys and for values."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def _check(t, name, dtype, *shape):
+    """A contiguous CUDA tensor of this dtype; None in `shape` stands for any size."""
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous CUDA tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if len(t.shape) != len(shape) or any(s is not None and s != have for s, have in zip(shape, t.shape)):
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+
+
+def _launch(first, others, name, *args):
+    """One C ABI call on `first`'s device and that device's current torch stream."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+    stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if torch.cuda.current_device() == dev.index:
+        call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream)
+
+
+def _float_kind(t, name):
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    return DTYPE["bf16" if t.dtype == torch.bfloat16 else "f32"]
+
+
+def quantize_rows_e4m3(x):
+    """Rows of x [m, d] (fp32 or bf16) as e4m3 codes [m, d] with one scale each [m]:
+    scale = max |row| / 448, x ~ codes * scale."""
+    kind = _float_kind(x, "x")
+    _check(x, "x", x.dtype, None, None)
+    m, d = x.shape
+    q = torch.empty(m, d, dtype=F8, device=x.device)
+    scale = torch.empty(m, dtype=torch.float32, device=x.device)
+    _launch(x, (), "fe_quantize_rows_e4m3", x.data_ptr(), kind, m, d, q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def add_rmsnorm_e4m3(y, h32, w, eps, one_plus=False):
+    """h32 += y in place (y fp32 or bf16, or None: no addition); returns RMSNorm(h32) * w
+    (1 + w when one_plus) as (e4m3 codes [m, d], scales [m])."""
+    _check(h32, "h32", torch.float32, None, None)
+    m, d = h32.shape
+    kind = DTYPE["f32"]
+    if y is not None:
+        kind = _float_kind(y, "y")
+        _check(y, "y", y.dtype, m, d)
+    _check(w, "w", torch.float32, d)
+    q = torch.empty(m, d, dtype=F8, device=h32.device)
+    scale = torch.empty(m, dtype=torch.float32, device=h32.device)
+    _launch(h32, (y, w), "fe_add_rmsnorm_e4m3", None if y is None else y.data_ptr(), kind, h32.data_ptr(), w.data_ptr(),
+            1 if one_plus else 0, eps, m, d, q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def linear_e4m3(x, x_scale, w, w_scale, bias=None, residual=None, epilogue="none", out_dtype="bf16"):
+    """y = epilogue((x * x_scale[:, None]) @ (w * w_scale[:, None]).T): x [m, k] and w [n, k] e4m3
+    codes with one scale per row (quantize_rows_e4m3, add_rmsnorm_e4m3)."""
+    _check(x, "x", F8, None, None)
+    m, k = x.shape
+    _check(w, "w", F8, None, k)
+    n = w.shape[0]
+    _check(x_scale, "x_scale", torch.float32, m)
+    _check(w_scale, "w_scale", torch.float32, n)
+    if bias is not None:
+        _check(bias, "bias", torch.float32, n)
+    if residual is not None:
+        _check(residual, "residual", torch.float32, m, n)
+    ny = n // 2 if epilogue in ("swiglu", "geglu") else n
+    y = torch.empty(m, ny, dtype=torch.bfloat16 if out_dtype == "bf16" else torch.float32, device=x.device)
+    _launch(x, (x_scale, w, w_scale, bias, residual), "fe_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), w.data_ptr(),
+            w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(), y.data_ptr(), m, n, k, EPI[epilogue], DTYPE[out_dtype])
+    return y
+
+
+def kv_cache_e4m3(pages, page_size, kv_heads, head_dim, device):
+    """An empty cache of `pages` pages."""
+    shape = (pages, kv_heads, page_size, head_dim)
+    return KvCacheE4m3(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(F8) for _ in range(2)),
+                       *(torch.zeros(pages, kv_heads, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads):
+    """Checks the arguments that the cache's write and its attention share; (batch, kv_heads,
+    head_dim, table width, pages, page size)."""
+    _check(cache.k, "cache.k", F8, None, None, None, None)
+    pages, kv_heads, page, hd = cache.k.shape
+    _check(cache.v, "cache.v", F8, pages, kv_heads, page, hd)
+    _check(cache.k_scale, "cache.k_scale", torch.float32, pages, kv_heads)
+    _check(cache.v_scale, "cache.v_scale", torch.float32, pages, kv_heads)
+    _check(qkv, "qkv", torch.bfloat16, None, (q_heads + 2 * kv_heads) * hd)
+    _check(cu_seqlens, "cu_seqlens", torch.int32, None)
+    batch = cu_seqlens.numel() - 1
+    if batch < 0:
+        raise ValueError("cu_seqlens: expected batch + 1 offsets")
+    _check(past_lens, "past_lens", torch.int32, batch)
+    _check(page_table, "page_table", torch.int32, batch, None)
+    return batch, kv_heads, hd, page_table.shape[1], pages, page
+
+
+def kv_cache_append_e4m3(qkv, cu_seqlens, max_len, past_lens, page_table, cache, q_heads):
+    """Writes the keys and values of the packed new tokens qkv [T, (Hq + 2 Hkv) * hd] (bf16) into
+    the cache: token i of sequence b at position past_lens[b] + i, in page
+    page_table[b, position // page_size].  In place."""
+    batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
+    _launch(qkv, (cu_seqlens, past_lens, page_table, *cache), "fe_kv_cache_append_e4m3", qkv.data_ptr(),
+            cu_seqlens.data_ptr(), batch, max_len, qkv.shape[0], q_heads, kv_heads, hd, past_lens.data_ptr(),
+            page_table.data_ptr(), width, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), pages, page)
+    return cache
+
+
+def attention_cache_e4m3(qkv, cu_seqlens, max_len, past_lens, max_kv_len, page_table, cache, q_heads, causal=True,
+                         scale=None, out=None):
+    """Attention of the packed new tokens over their sequences' cache (after
+    kv_cache_append_e4m3): [T, Hq * hd] bf16.  max_kv_len bounds past_lens + new tokens.  A given
+    `out` keeps the rows that belong to no sequence."""
+    batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
+    T = qkv.shape[0]
+    scale = hd ** -0.5 if scale is None else scale
+    if out is None:
+        out = torch.empty(T, q_heads * hd, dtype=torch.bfloat16, device=qkv.device)
+    else:
+        _check(out, "out", torch.bfloat16, T, q_heads * hd)
+    size = C.c_size_t(0)
+    dev = qkv.device
+    with torch.cuda.device(dev):  # the split goes by the device's SM count
+        call("fe_attention_cache_workspace_bytes", batch, max_len, T, max_kv_len, q_heads, kv_heads, hd, C.byref(size))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
+    _launch(qkv, (cu_seqlens, past_lens, page_table, out, *cache), "fe_attention_cache_e4m3", qkv.data_ptr(),
+            cu_seqlens.data_ptr(), batch, max_len, T, q_heads, kv_heads, hd, past_lens.data_ptr(), max_kv_len,
+            page_table.data_ptr(), width, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), pages, page, 1 if causal else 0, scale, out.data_ptr(),
+            None if ws is None else ws.data_ptr(), size.value)
     return out
 
 

@@ -296,6 +296,77 @@ fe_status fe_qk_norm_rope_bf16(void *qkv, const int32_t *cu_seqlens, int32_t bat
 fe_status fe_pool_l2(const float *h, const int32_t *cu_seqlens, int32_t batch, int32_t dim,
                      fe_pooling mode, float *out, fe_stream_t stream);
 
+/* ------------------------------------------------------ 8-bit operators -----
+ * The serving path of the RMSNorm encoders with e4m3 operands (OCP 8-bit floats: 4 exponent
+ * and 3 mantissa bits, largest value 448): the row quantisers, the linear layer over their
+ * codes, and a paged key-value cache with the attention that reads it, for encoders whose
+ * inputs share a prefix (an instruction, a document's earlier part).  Not in the reference
+ * (its arithmetic is fp32 and it caches nothing).  A quantised value is code * scale.
+ * Stream-ordered like every op: no allocation, no synchronisation; all can be captured into a
+ * CUDA graph once the device's status word exists (call fe_device_status(device) first). */
+
+/* Rows to e4m3: scale[i] = max(max_j |x[i][j]|, 2^-110) / 448 over the finite elements,
+ * q[i][j] = e4m3(x[i][j] / scale[i]); a non-finite element takes the NaN code.  x is fp32 or
+ * bf16 [rows, dim], q one byte per element.  Any dim; 16-byte aligned rows of a multiple of 8
+ * elements take the faster kernels. */
+fe_status fe_quantize_rows_e4m3(const void *x, fe_dtype x_dtype, int64_t rows, int32_t dim, void *q, float *scale,
+                                fe_stream_t stream);
+/* h32 += y in place (y fp32 or bf16 [rows, dim]; NULL: no addition, h32 is not written), then
+ * RMSNorm(h32) = h32 / sqrt(mean(h32^2) + eps) * w (1 + w when one_plus) as fe_quantize_rows_e4m3
+ * of its rows, normalised in fp32. */
+fe_status fe_add_rmsnorm_e4m3(const void *y, fe_dtype y_dtype, float *h32, const float *w, int32_t one_plus, float eps,
+                              int64_t rows, int32_t dim, void *q, float *scale, fe_stream_t stream);
+/* y[m,n] = epilogue(x_scale[i] * w_scale[j] * (x[m,k] . w[n,k]^T)) over e4m3 codes, one scale
+ * per row of x and of w, FP32 accumulation; the epilogues of fe_linear_bf16, gated ones included.
+ * y is bf16 or fp32; activations and gates write bf16, the residual form fp32 (y may be the
+ * residual itself).  k % 16 == 0, n % 8 == 0; 16-byte aligned pointers (x_scale: 4). */
+fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, const float *w_scale, const float *bias,
+                         const float *residual, void *y, int64_t m, int64_t n, int64_t k, fe_epilogue epilogue,
+                         fe_dtype y_dtype, fe_stream_t stream);
+
+/* The cache: k_pages and v_pages hold `pages` pages of page_size (16, 32, 64 or 128) tokens as
+ * e4m3 codes [pages, kv_heads, page_size, head_dim]; k_scales and v_scales one fp32 scale per
+ * page and head [pages, kv_heads].  Token p of sequence b lies in page
+ * page_table[b][p / page_size], slot p % page_size (page_table device int32 [batch,
+ * table_width]).  The batch is packed like fe_attention_varlen_gqa_bf16's: qkv bf16
+ * [total_tokens, (q_heads + 2 kv_heads) * head_dim], rows cu_seqlens[b] .. cu_seqlens[b+1] the
+ * new tokens of sequence b (at most max_len), at positions past_lens[b] and up.  head_dim 64,
+ * 128 or 256.  cu_seqlens, past_lens and page_table are read on the device: a sequence whose
+ * offsets do not fit (rows past total_tokens, more than max_len or table_width pages of tokens,
+ * a negative past) is left out, and so are the tokens of a page id outside [0, pages); either
+ * sets FE_ERR_INVALID_ARGUMENT in the device status word. */
+
+/* Writes the new tokens' keys and values into their pages.  The scale of a (page, head) is the
+ * smallest power of two s >= 2^-80 with max |v| <= 448 s over the finite values written to the
+ * page so far (0 if all are zero); when new tokens raise it, the page's older codes are
+ * re-encoded.  The page of slot 0 starts afresh, whatever it held.  A token with a non-finite
+ * key or value element of a head stores NaN as all of that key (and 0 for such value elements):
+ * queries that see it get NaN.  A page that two sequences share may be read by both but must
+ * not be reached by new tokens of more than one of them in one call. */
+fe_status fe_kv_cache_append_e4m3(const void *qkv, const int32_t *cu_seqlens, int32_t batch, int32_t max_len,
+                                  int64_t total_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                  const int32_t *past_lens, const int32_t *page_table, int32_t table_width, void *k_pages,
+                                  void *v_pages, float *k_scales, float *v_scales, int32_t pages, int32_t page_size,
+                                  fe_stream_t stream);
+/* Bytes of device workspace fe_attention_cache_e4m3 needs for the same arguments (may be 0). */
+fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int64_t total_tokens, int32_t max_kv_len,
+                                             int32_t q_heads, int32_t kv_heads, int32_t head_dim, size_t *bytes);
+/* Attention of the new tokens over their sequence's cache, after fe_kv_cache_append_e4m3 with
+ * the same batch: out [total_tokens, q_heads * head_dim] bf16 = softmax(Q K^T * scale) V, query
+ * i of sequence b seeing the cached tokens j <= past_lens[b] + i (causal != 0) or all
+ * past_lens[b] + len of them.  Query head h reads key-value head h / (q_heads / kv_heads).
+ * max_kv_len is the caller's bound on past_lens[b] + len: it decides how sequences are split
+ * over CTAs, not what is read.  Rows of out that belong to no sequence are left as they are; a
+ * row that sees nothing (its pages are all out of range) is zero.  Scales may be any finite
+ * positive numbers or 0; value codes of visible tokens must not be NaN (append writes none).
+ * Calls that share a workspace must not run concurrently; its contents need no initialisation. */
+fe_status fe_attention_cache_e4m3(const void *qkv, const int32_t *cu_seqlens, int32_t batch, int32_t max_len,
+                                  int64_t total_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                  const int32_t *past_lens, int32_t max_kv_len, const int32_t *page_table,
+                                  int32_t table_width, const void *k_pages, const void *v_pages, const float *k_scales,
+                                  const float *v_scales, int32_t pages, int32_t page_size, int32_t causal, float scale,
+                                  void *out, void *workspace, size_t workspace_bytes, fe_stream_t stream);
+
 /* --------------------------------------------------------- model engine
  * Device-resident post-LN BERT encoder (the reference's bge_forward,
  * src/sentence_transformers_impl.cpp:126-344, batched and packed). */
