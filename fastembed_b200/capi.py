@@ -147,7 +147,9 @@ def check(status: int, where: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status != FE_OK:
+        check(status, name)
 
 
 def exported_symbols() -> list[str]:

@@ -45,6 +45,14 @@ fe_status check_cache(const char *name, int32_t batch, int32_t max_len, int64_t 
     return FE_OK;
 }
 
+// What a call that has work to do needs of the pool: TMA coordinates count its rows in 32 bits.
+fe_status check_pool(const char *name, int32_t pages, int32_t kv_heads, int32_t page)
+{
+    if (pages == 0) return bad(name, "a pool without pages");
+    if (static_cast<int64_t>(pages) * kv_heads * page > 0x7ffffff0) return unsupported(name, "pages x kv_heads x page_size past 2^31");
+    return FE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -110,6 +118,7 @@ fe_status fe_kv_cache_append_e4m3(const void *qkv, const int32_t *cu_seqlens, in
     const char *name = "fe_kv_cache_append_e4m3";
     FE_TRY(check_cache(name, batch, max_len, total_tokens, q_heads, kv_heads, head_dim, table_width, pages, page_size));
     if (batch == 0 || total_tokens == 0 || max_len == 0) return FE_OK;
+    FE_TRY(check_pool(name, pages, kv_heads, page_size));
     if (!qkv || !cu_seqlens || !past_lens || !page_table || !k_pages || !v_pages || !k_scales || !v_scales)
         return bad(name, "null pointer");
     if (!aligned16(qkv) || !aligned16(k_pages) || !aligned16(v_pages)) return bad(name, "pointers must be 16-byte aligned");
@@ -144,6 +153,7 @@ fe_status fe_attention_cache_e4m3(const void *qkv, const int32_t *cu_seqlens, in
     FE_TRY(check_cache(name, batch, max_len, total_tokens, q_heads, kv_heads, head_dim, table_width, pages, page_size));
     if (max_kv_len < 0 || !std::isfinite(scale)) return bad(name, "bad max_kv_len or scale");
     if (batch == 0 || total_tokens == 0 || max_len == 0) return FE_OK;
+    FE_TRY(check_pool(name, pages, kv_heads, page_size));
     if (!qkv || !cu_seqlens || !past_lens || !page_table || !k_pages || !v_pages || !k_scales || !v_scales || !out)
         return bad(name, "null pointer");
     if (!aligned16(qkv) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out))
@@ -152,11 +162,13 @@ fe_status fe_attention_cache_e4m3(const void *qkv, const int32_t *cu_seqlens, in
         fe::attention_cache_workspace_bytes(batch, max_len, total_tokens, max_kv_len, q_heads, kv_heads, head_dim);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return bad(name, "workspace missing, too small or not 16-byte aligned");
-    return fe::check_cuda(
-        fe::launch_attention_cache_e4m3(qkv, cu_seqlens, batch, max_len, total_tokens, q_heads, kv_heads, head_dim, past_lens,
-                                        max_kv_len, page_table, table_width, k_pages, v_pages, k_scales, v_scales, pages,
-                                        page_size, causal != 0, scale, out, workspace, cs(stream)),
-        name);
+    fe_status st = FE_OK;
+    cudaError_t e = fe::launch_attention_cache_e4m3(qkv, cu_seqlens, batch, max_len, total_tokens, q_heads, kv_heads, head_dim,
+                                                    past_lens, max_kv_len, page_table, table_width, k_pages, v_pages, k_scales,
+                                                    v_scales, pages, page_size, causal != 0, scale, out, workspace, cs(stream),
+                                                    &st);
+    if (st != FE_OK) return st;
+    return fe::check_cuda(e, name);
 }
 
 }  // extern "C"

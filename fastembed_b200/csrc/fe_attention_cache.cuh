@@ -1,0 +1,61 @@
+// fe_attention_cache.cuh — what the kernels of the attention over the paged 8-bit cache share:
+// arguments, the reading of a sequence's offsets, and the launcher of the tile kernel.
+#pragma once
+
+#include "fe_e4m3.cuh"
+#include "fe_internal.h"
+
+namespace fe {
+
+struct CacheArgs {
+    const __nv_bfloat16 *qkv;
+    const int32_t *cu, *past, *table;
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    __nv_bfloat16 *out;
+    float *part_o;  // [T * q_heads][splits][hd], splits > 1
+    float *part_ml; // [T * q_heads][splits][2]: reference exponent, sum
+    int64_t total, row;
+    int batch, max_len, width, pages, page_log2, q_heads, kv_heads, group, causal;
+    int splits;
+    float scale_log2;
+};
+
+// One sequence of the batch: false (and a report) when its offsets do not describe it.
+struct CacheSeq {
+    int t0, len, past, kv;  // first row, new tokens, tokens before them, tokens in the cache
+};
+
+__device__ __forceinline__ bool load_seq(const CacheArgs &a, int b, CacheSeq &s, int *status)
+{
+    s.t0 = a.cu[b];
+    const int t1 = a.cu[b + 1];
+    s.past = a.past[b];
+    s.len = t1 - s.t0;
+    if (s.len <= 0) return false;
+    const int64_t kv = static_cast<int64_t>(s.past) + s.len;
+    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 &&
+                    kv <= (static_cast<int64_t>(a.width) << a.page_log2);
+    s.kv = static_cast<int>(kv);
+    if (!ok && threadIdx.x == 0) report(status, DEV_BAD_INPUT);
+    return ok;
+}
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Rows of a sequence's key-value head (tokens x query heads of its group) per unit of the tile kernel.
+int attention_cache_tile_rows(int head_dim);
+cudaError_t launch_attention_cache_tiles(const CacheArgs &a, int head_dim, int *status, cudaStream_t s, fe_status *st);
+
+}  // namespace fe

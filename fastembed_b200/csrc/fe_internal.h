@@ -49,6 +49,7 @@ cudaError_t set_wait_limit_linear(uint64_t ns);
 cudaError_t set_wait_limit_attention(uint64_t ns);
 cudaError_t set_wait_limit_attention_wide(uint64_t ns);
 cudaError_t set_wait_limit_linear_e4m3(uint64_t ns);
+cudaError_t set_wait_limit_attention_cache(uint64_t ns);
 int current_sm_count();
 // Programmatic dependent launch for the kernels that call grid_dep_wait(): on with
 // FE_PDL=1 (read once per process), off by default.  On bge-large, Qwen3- and
@@ -172,7 +173,7 @@ cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int 
                                         int q_heads, int kv_heads, int head_dim, const int32_t *past, int max_kv,
                                         const int32_t *table, int width, const void *k, const void *v, const float *ks,
                                         const float *vs, int pages, int page, bool causal, float scale, void *out,
-                                        void *workspace, cudaStream_t s);
+                                        void *workspace, cudaStream_t s, fe_status *st);
 
 cudaError_t launch_sgemm(const float *a, const float *b, const float *bias, float *c, int64_t m,
                          int64_t n, int64_t k, bool b_transposed, cudaStream_t s);

@@ -31,21 +31,14 @@
 // FE_ERR_INVALID_ARGUMENT in the device status word and its tokens are left out.
 #include <algorithm>
 
-#include "fe_e4m3.cuh"
-#include "fe_internal.h"
+#include "fe_attention_cache.cuh"
 
 namespace fe {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBoost = 15.f;  // P is at most 2^15
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+constexpr int kSms = 148;
 
 // D += A B, m16n8k16, f16 inputs, fp32 accumulator
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -63,12 +56,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v)
     return r;
 }
 
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
-{
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 __device__ __forceinline__ uint4 ld_stream16(const uint8_t *p)
 {
     uint4 v;
@@ -83,38 +70,6 @@ __device__ __forceinline__ uint2 ld_stream8(const uint8_t *p)
     uint2 v;
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
-}
-
-struct CacheArgs {
-    const __nv_bfloat16 *qkv;
-    const int32_t *cu, *past, *table;
-    const uint8_t *k, *v;
-    const float *ks, *vs;
-    __nv_bfloat16 *out;
-    float *part_o;  // [T * q_heads][splits][hd], splits > 1
-    float *part_ml; // [T * q_heads][splits][2]: m, l
-    int64_t total, row;
-    int batch, max_len, width, pages, page_log2, q_heads, kv_heads, group, causal;
-    int splits;
-    float scale_log2;
-};
-
-// One sequence of the batch: false (and a report) when its offsets do not describe it.
-struct Seq {
-    int t0, len, past, kv;  // first row, new tokens, tokens before them, tokens in the cache
-};
-__device__ __forceinline__ bool load_seq(const CacheArgs &a, int b, Seq &s, int *status)
-{
-    s.t0 = a.cu[b];
-    const int t1 = a.cu[b + 1];
-    s.past = a.past[b];
-    s.len = t1 - s.t0;
-    if (s.len <= 0) return false;
-    const int64_t kv = static_cast<int64_t>(s.past) + s.len;
-    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 && kv <= (static_cast<int64_t>(a.width) << a.page_log2);
-    s.kv = static_cast<int>(kv);
-    if (!ok && threadIdx.x == 0) report(status, DEV_BAD_INPUT);
-    return ok;
 }
 
 constexpr int kWarpTokens = 32;
@@ -143,7 +98,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     const int b = blockIdx.x / row_tiles, tile = blockIdx.x % row_tiles;
     grid_dep_wait();
     grid_dep_launch();
-    Seq sq;
+    CacheSeq sq;
     if (!load_seq(a, b, sq, status)) return;
     const int rows = sq.len * a.group, r0 = tile * C::ROWS;
     if (r0 >= rows) return;
@@ -452,7 +407,7 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
     const int lane = threadIdx.x & 31;
     grid_dep_wait();
     grid_dep_launch();
-    Seq sq;
+    CacheSeq sq;
     if (!load_seq(a, blockIdx.y, sq, status)) return;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     if (i >= static_cast<int64_t>(sq.len) * a.q_heads) return;
@@ -478,7 +433,20 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
     for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
+template <int HD>
+cudaError_t launch_join(const CacheArgs &a, int *status, cudaStream_t s)
+{
+    return launch_k(attn_cache_join<HD>, dim3((static_cast<unsigned>(a.max_len) * a.q_heads + 3) / 4, a.batch), dim3(128), 0,
+                    s, a, status);
+}
+
+cudaError_t launch_join(const CacheArgs &a, int head_dim, int *status, cudaStream_t s)
+{
+    return head_dim == 64 ? launch_join<64>(a, status, s) : head_dim == 128 ? launch_join<128>(a, status, s) : launch_join<256>(a, status, s);
+}
+
 constexpr int kWarps = 4;
+constexpr int kStreamRows = 32;  // rows of a key-value head up to which the streaming kernel runs
 
 // 8-row tiles of a CTA: 16 rows where the registers allow it and there are more than 8
 int row_tile_count(int rows, int head_dim) { return rows > 8 && head_dim < 256 ? 2 : 1; }
@@ -492,9 +460,7 @@ cudaError_t stream(const CacheArgs &a, int *status, cudaStream_t s)
     cudaError_t e = launch_k(attn_cache_stream<HD, NR, kWarps>,
                              dim3(static_cast<unsigned>(a.batch) * row_tiles, a.kv_heads, a.splits), dim3(32 * kWarps),
                              C::SMEM, s, a, row_tiles, status);
-    if (e != cudaSuccess || a.splits == 1) return e;
-    return launch_k(attn_cache_join<HD>, dim3((static_cast<unsigned>(a.max_len) * a.q_heads + 3) / 4, a.batch), dim3(128), 0,
-                    s, a, status);
+    return e != cudaSuccess || a.splits == 1 ? e : launch_join<HD>(a, status, s);
 }
 
 template <int HD>
@@ -507,21 +473,36 @@ cudaError_t stream_any(const CacheArgs &a, int *status, cudaStream_t s)
 
 }  // namespace
 
-// Parts the sequences are split into: enough CTAs for about four rounds of the resident ones
-// (sequences differ in length), each with 512 tokens or more of the longest.
-int attention_cache_splits(int batch, int max_len, int max_kv, int q_heads, int kv_heads, int head_dim)
+// Which kernel runs and into how many parts the sequences are split.  A matter of the arguments
+// alone (a B200 has kSms multiprocessors), so that a workspace sized on one device serves on any.
+struct CachePlan {
+    bool tiles;
+    int splits;
+};
+CachePlan plan_attention_cache(int batch, int max_len, int max_kv, int q_heads, int kv_heads, int head_dim)
 {
     const int64_t rows = static_cast<int64_t>(max_len) * (q_heads / kv_heads);
-    const int per = 8 * row_tile_count(static_cast<int>(std::min<int64_t>(rows, 1 << 20)), head_dim);
-    const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
-    const int64_t want = (12ll * current_sm_count() + ctas - 1) / ctas;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+    CachePlan p;
+    p.tiles = rows > kStreamRows;
+    int64_t want;
+    if (p.tiles) {
+        const int64_t tiles = (rows + attention_cache_tile_rows(head_dim) - 1) / attention_cache_tile_rows(head_dim);
+        // one CTA an SM: split until they have one each, 512 tokens or more a part
+        want = std::min<int64_t>(kSms / std::max<int64_t>(1, tiles * batch * kv_heads), 65535 / tiles);
+    } else {
+        // enough CTAs for about four rounds of the resident ones (sequences differ in length)
+        const int per = 8 * row_tile_count(static_cast<int>(rows), head_dim);
+        const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
+        want = (12ll * kSms + ctas - 1) / ctas;
+    }
+    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+    return p;
 }
 
 size_t attention_cache_workspace_bytes(int batch, int max_len, int64_t total, int max_kv, int q_heads, int kv_heads,
                                        int head_dim)
 {
-    const int64_t splits = attention_cache_splits(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    const int64_t splits = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim).splits;
     return splits == 1 ? 0 : static_cast<size_t>(total) * q_heads * splits * (head_dim + 2) * sizeof(float);
 }
 
@@ -529,8 +510,9 @@ cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int 
                                         int q_heads, int kv_heads, int head_dim, const int32_t *past, int max_kv,
                                         const int32_t *table, int width, const void *k, const void *v, const float *ks,
                                         const float *vs, int pages, int page, bool causal, float scale, void *out,
-                                        void *workspace, cudaStream_t s)
+                                        void *workspace, cudaStream_t s, fe_status *st)
 {
+    *st = FE_OK;
     CacheArgs a;
     a.qkv = static_cast<const __nv_bfloat16 *>(qkv);
     a.cu = cu, a.past = past, a.table = table;
@@ -543,10 +525,15 @@ cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int 
     a.page_log2 = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
     a.q_heads = q_heads, a.kv_heads = kv_heads, a.group = q_heads / kv_heads, a.causal = causal;
     a.scale_log2 = scale * kLog2e;
-    a.splits = attention_cache_splits(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    const CachePlan plan = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    a.splits = plan.splits;
     a.part_o = static_cast<float *>(workspace);
     a.part_ml = a.part_o + total * q_heads * a.splits * head_dim;
     int *status = current_device_status_word();
+    if (plan.tiles) {
+        cudaError_t e = launch_attention_cache_tiles(a, head_dim, status, s, st);
+        return e != cudaSuccess || *st != FE_OK || a.splits == 1 ? e : launch_join(a, head_dim, status, s);
+    }
     if (head_dim == 64) return stream_any<64>(a, status, s);
     if (head_dim == 128) return stream_any<128>(a, status, s);
     return stream_any<256>(a, status, s);

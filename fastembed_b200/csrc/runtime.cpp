@@ -223,6 +223,7 @@ fe_status fe_set_wait_limit(int device, uint64_t limit_ns)
     if (e == cudaSuccess) e = fe::set_wait_limit_attention(limit_ns);
     if (e == cudaSuccess) e = fe::set_wait_limit_attention_wide(limit_ns);
     if (e == cudaSuccess) e = fe::set_wait_limit_linear_e4m3(limit_ns);
+    if (e == cudaSuccess) e = fe::set_wait_limit_attention_cache(limit_ns);
     cudaSetDevice(prev);
     return fe::check_cuda(e, "fe_set_wait_limit");
 }

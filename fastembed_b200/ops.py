@@ -295,83 +295,91 @@ class KvCacheE4m3(NamedTuple):
     v_scale: torch.Tensor
 
 
-def _check(t, name, dtype, *shape):
-    """A contiguous CUDA tensor of this dtype; None in `shape` stands for any size."""
+def _why(t, name, dtype, shape, dev):
     if not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous CUDA tensor")
+        return f"{name}: expected a contiguous CUDA tensor"
+    if t.get_device() != dev:
+        return f"{name}: expected a tensor on cuda:{dev}, got {t.device}"
     if t.dtype != dtype:
-        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
-    if len(t.shape) != len(shape) or any(s is not None and s != have for s, have in zip(shape, t.shape)):
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+        return f"{name}: expected {dtype}, got {t.dtype}"
+    return f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}"
 
 
-def _launch(first, others, name, *args):
-    """One C ABI call on `first`'s device and that device's current torch stream."""
-    dev = first.device
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
-    stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if torch.cuda.current_device() == dev.index:
+def _check(t, name, dtype, shape, dev):
+    """A contiguous tensor of this dtype and shape on CUDA device `dev`.  (These calls last a few
+    microseconds on the GPU for single tokens, so the front end counts: the checks are four
+    attribute comparisons and the message is made only when one fails.)"""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous() or dev < 0:
+        raise ValueError(_why(t, name, dtype, shape, dev))
+
+
+def _matrix(t, name, dtype=None):
+    """(device, rows, columns) of a contiguous 2-D CUDA tensor of this dtype (None: fp32 or bf16)."""
+    if dtype is None and t.dtype is not torch.float32 and t.dtype is not torch.bfloat16:
+        raise ValueError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected a matrix, got shape {tuple(t.shape)}")
+    dev = t.get_device()
+    _check(t, name, dtype or t.dtype, t.shape, dev)
+    return dev, *t.shape
+
+
+def _launch(dev, name, *args):
+    """One C ABI call on CUDA device `dev` and that device's current torch stream."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without its Stream object
+    if torch.cuda.current_device() == dev:
         call(name, *args, stream)
     else:
         with torch.cuda.device(dev):
             call(name, *args, stream)
 
 
-def _float_kind(t, name):
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
-    return DTYPE["bf16" if t.dtype == torch.bfloat16 else "f32"]
+_KIND = {torch.float32: DTYPE["f32"], torch.bfloat16: DTYPE["bf16"]}
+_OUT = {"bf16": torch.bfloat16, "f32": torch.float32}
 
 
 def quantize_rows_e4m3(x):
     """Rows of x [m, d] (fp32 or bf16) as e4m3 codes [m, d] with one scale each [m]:
     scale = max |row| / 448, x ~ codes * scale."""
-    kind = _float_kind(x, "x")
-    _check(x, "x", x.dtype, None, None)
-    m, d = x.shape
-    q = torch.empty(m, d, dtype=F8, device=x.device)
+    dev, m, d = _matrix(x, "x")
+    q = torch.empty_like(x, dtype=F8)
     scale = torch.empty(m, dtype=torch.float32, device=x.device)
-    _launch(x, (), "fe_quantize_rows_e4m3", x.data_ptr(), kind, m, d, q.data_ptr(), scale.data_ptr())
+    _launch(dev, "fe_quantize_rows_e4m3", x.data_ptr(), _KIND[x.dtype], m, d, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
 def add_rmsnorm_e4m3(y, h32, w, eps, one_plus=False):
     """h32 += y in place (y fp32 or bf16, or None: no addition); returns RMSNorm(h32) * w
     (1 + w when one_plus) as (e4m3 codes [m, d], scales [m])."""
-    _check(h32, "h32", torch.float32, None, None)
-    m, d = h32.shape
-    kind = DTYPE["f32"]
+    dev, m, d = _matrix(h32, "h32", torch.float32)
     if y is not None:
-        kind = _float_kind(y, "y")
-        _check(y, "y", y.dtype, m, d)
-    _check(w, "w", torch.float32, d)
-    q = torch.empty(m, d, dtype=F8, device=h32.device)
+        if y.dtype not in _KIND:
+            raise ValueError(f"y: expected float32 or bfloat16, got {y.dtype}")
+        _check(y, "y", y.dtype, h32.shape, dev)
+    _check(w, "w", torch.float32, (d,), dev)
+    q = torch.empty_like(h32, dtype=F8)
     scale = torch.empty(m, dtype=torch.float32, device=h32.device)
-    _launch(h32, (y, w), "fe_add_rmsnorm_e4m3", None if y is None else y.data_ptr(), kind, h32.data_ptr(), w.data_ptr(),
-            1 if one_plus else 0, eps, m, d, q.data_ptr(), scale.data_ptr())
+    _launch(dev, "fe_add_rmsnorm_e4m3", None if y is None else y.data_ptr(), 0 if y is None else _KIND[y.dtype],
+            h32.data_ptr(), w.data_ptr(), 1 if one_plus else 0, eps, m, d, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
 def linear_e4m3(x, x_scale, w, w_scale, bias=None, residual=None, epilogue="none", out_dtype="bf16"):
     """y = epilogue((x * x_scale[:, None]) @ (w * w_scale[:, None]).T): x [m, k] and w [n, k] e4m3
     codes with one scale per row (quantize_rows_e4m3, add_rmsnorm_e4m3)."""
-    _check(x, "x", F8, None, None)
-    m, k = x.shape
-    _check(w, "w", F8, None, k)
+    dev, m, k = _matrix(x, "x", F8)
     n = w.shape[0]
-    _check(x_scale, "x_scale", torch.float32, m)
-    _check(w_scale, "w_scale", torch.float32, n)
+    _check(w, "w", F8, (n, k), dev)
+    _check(x_scale, "x_scale", torch.float32, (m,), dev)
+    _check(w_scale, "w_scale", torch.float32, (n,), dev)
     if bias is not None:
-        _check(bias, "bias", torch.float32, n)
+        _check(bias, "bias", torch.float32, (n,), dev)
     if residual is not None:
-        _check(residual, "residual", torch.float32, m, n)
-    ny = n // 2 if epilogue in ("swiglu", "geglu") else n
-    y = torch.empty(m, ny, dtype=torch.bfloat16 if out_dtype == "bf16" else torch.float32, device=x.device)
-    _launch(x, (x_scale, w, w_scale, bias, residual), "fe_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), w.data_ptr(),
-            w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), y.data_ptr(), m, n, k, EPI[epilogue], DTYPE[out_dtype])
+        _check(residual, "residual", torch.float32, (m, n), dev)
+    y = torch.empty((m, n // 2 if epilogue in ("swiglu", "geglu") else n), dtype=_OUT[out_dtype], device=x.device)
+    _launch(dev, "fe_linear_e4m3", x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+            None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), m, n,
+            k, EPI[epilogue], DTYPE[out_dtype])
     return y
 
 
@@ -383,32 +391,38 @@ def kv_cache_e4m3(pages, page_size, kv_heads, head_dim, device):
 
 
 def _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads):
-    """Checks the arguments that the cache's write and its attention share; (batch, kv_heads,
-    head_dim, table width, pages, page size)."""
-    _check(cache.k, "cache.k", F8, None, None, None, None)
-    pages, kv_heads, page, hd = cache.k.shape
-    _check(cache.v, "cache.v", F8, pages, kv_heads, page, hd)
-    _check(cache.k_scale, "cache.k_scale", torch.float32, pages, kv_heads)
-    _check(cache.v_scale, "cache.v_scale", torch.float32, pages, kv_heads)
-    _check(qkv, "qkv", torch.bfloat16, None, (q_heads + 2 * kv_heads) * hd)
-    _check(cu_seqlens, "cu_seqlens", torch.int32, None)
-    batch = cu_seqlens.numel() - 1
+    """Checks the arguments that the cache's write and its attention share; (device, rows, batch,
+    kv_heads, head_dim, table width, pages, page size)."""
+    k, v, ks, vs = cache
+    dev = k.get_device()
+    if k.dim() != 4:
+        raise ValueError(f"cache.k: expected [pages, kv_heads, page_size, head_dim], got {tuple(k.shape)}")
+    pages, kv_heads, page, hd = k.shape
+    _check(k, "cache.k", F8, k.shape, dev)
+    _check(v, "cache.v", F8, k.shape, dev)
+    _check(ks, "cache.k_scale", torch.float32, (pages, kv_heads), dev)
+    _check(vs, "cache.v_scale", torch.float32, (pages, kv_heads), dev)
+    T = qkv.shape[0]
+    _check(qkv, "qkv", torch.bfloat16, (T, (q_heads + 2 * kv_heads) * hd), dev)
+    batch = cu_seqlens.shape[0] - 1
     if batch < 0:
         raise ValueError("cu_seqlens: expected batch + 1 offsets")
-    _check(past_lens, "past_lens", torch.int32, batch)
-    _check(page_table, "page_table", torch.int32, batch, None)
-    return batch, kv_heads, hd, page_table.shape[1], pages, page
+    width = page_table.shape[-1]
+    _check(cu_seqlens, "cu_seqlens", torch.int32, (batch + 1,), dev)
+    _check(past_lens, "past_lens", torch.int32, (batch,), dev)
+    _check(page_table, "page_table", torch.int32, (batch, width), dev)
+    return dev, T, batch, kv_heads, hd, width, pages, page
 
 
 def kv_cache_append_e4m3(qkv, cu_seqlens, max_len, past_lens, page_table, cache, q_heads):
     """Writes the keys and values of the packed new tokens qkv [T, (Hq + 2 Hkv) * hd] (bf16) into
     the cache: token i of sequence b at position past_lens[b] + i, in page
     page_table[b, position // page_size].  In place."""
-    batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
-    _launch(qkv, (cu_seqlens, past_lens, page_table, *cache), "fe_kv_cache_append_e4m3", qkv.data_ptr(),
-            cu_seqlens.data_ptr(), batch, max_len, qkv.shape[0], q_heads, kv_heads, hd, past_lens.data_ptr(),
-            page_table.data_ptr(), width, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), pages, page)
+    dev, T, batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
+    k, v, ks, vs = cache
+    _launch(dev, "fe_kv_cache_append_e4m3", qkv.data_ptr(), cu_seqlens.data_ptr(), batch, max_len, T, q_heads, kv_heads, hd,
+            past_lens.data_ptr(), page_table.data_ptr(), width, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+            pages, page)
     return cache
 
 
@@ -417,23 +431,20 @@ def attention_cache_e4m3(qkv, cu_seqlens, max_len, past_lens, max_kv_len, page_t
     """Attention of the packed new tokens over their sequences' cache (after
     kv_cache_append_e4m3): [T, Hq * hd] bf16.  max_kv_len bounds past_lens + new tokens.  A given
     `out` keeps the rows that belong to no sequence."""
-    batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
-    T = qkv.shape[0]
-    scale = hd ** -0.5 if scale is None else scale
+    dev, T, batch, kv_heads, hd, width, pages, page = _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads)
+    k, v, ks, vs = cache
     if out is None:
-        out = torch.empty(T, q_heads * hd, dtype=torch.bfloat16, device=qkv.device)
+        out = torch.empty((T, q_heads * hd), dtype=torch.bfloat16, device=qkv.device)
     else:
-        _check(out, "out", torch.bfloat16, T, q_heads * hd)
+        _check(out, "out", torch.bfloat16, (T, q_heads * hd), dev)
     size = C.c_size_t(0)
-    dev = qkv.device
-    with torch.cuda.device(dev):  # the split goes by the device's SM count
-        call("fe_attention_cache_workspace_bytes", batch, max_len, T, max_kv_len, q_heads, kv_heads, hd, C.byref(size))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-    _launch(qkv, (cu_seqlens, past_lens, page_table, out, *cache), "fe_attention_cache_e4m3", qkv.data_ptr(),
-            cu_seqlens.data_ptr(), batch, max_len, T, q_heads, kv_heads, hd, past_lens.data_ptr(), max_kv_len,
-            page_table.data_ptr(), width, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), pages, page, 1 if causal else 0, scale, out.data_ptr(),
-            None if ws is None else ws.data_ptr(), size.value)
+    call("fe_attention_cache_workspace_bytes", batch, max_len, T, max_kv_len, q_heads, kv_heads, hd, C.byref(size))
+    size = size.value
+    ws = torch.empty(size, dtype=torch.uint8, device=qkv.device) if size else None
+    _launch(dev, "fe_attention_cache_e4m3", qkv.data_ptr(), cu_seqlens.data_ptr(), batch, max_len, T, q_heads, kv_heads, hd,
+            past_lens.data_ptr(), max_kv_len, page_table.data_ptr(), width, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+            vs.data_ptr(), pages, page, 1 if causal else 0, hd ** -0.5 if scale is None else scale, out.data_ptr(),
+            ws.data_ptr() if size else None, size)
     return out
 
 

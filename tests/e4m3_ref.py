@@ -94,13 +94,15 @@ def append(cache, qkv, new, past, table, q_heads):
 
 
 def attention(cache, qkv, new, past, table, q_heads, causal, scale):
-    """(out, sum_j p |v|, largest scale * sum_d |q k|) per (token, head) in 64 bits."""
+    """(out, sum_j p |v|, largest scale * sum_d |q k|, floor) per (token, head) in 64 bits; floor: the
+    row's largest weight as it meets the codes (p times the page's value scale) times sum_j |codes|."""
     pages, hkv, page, hd = cache.k.shape
     group = q_heads // hkv
     x = qkv.view(qkv.shape[0], -1, hd)[:, :q_heads].double()
     T = sum(new)
     out = torch.zeros(T, q_heads, hd, dtype=torch.float64, device=qkv.device)
-    mag, dot = torch.zeros_like(out), torch.zeros(T, q_heads, dtype=torch.float64, device=qkv.device)
+    mag, floor = torch.zeros_like(out), torch.zeros_like(out)
+    dot = torch.zeros(T, q_heads, dtype=torch.float64, device=qkv.device)
     t0 = 0
     for b, (n, p) in enumerate(zip(new, past)):
         if n == 0:
@@ -109,6 +111,8 @@ def attention(cache, qkv, new, past, table, q_heads, causal, scale):
         k = values(cache.k.view(torch.uint8)[at].view(F8), cache.k_scale[at]).transpose(0, 1).reshape(hkv, -1, hd)[:, :n + p]
         v = values(cache.v.view(torch.uint8)[at].view(F8), cache.v_scale[at]).transpose(0, 1).reshape(hkv, -1, hd)[:, :n + p]
         k, v = k.repeat_interleave(group, 0), v.repeat_interleave(group, 0)
+        sv = cache.v_scale[at].double().t().repeat_interleave(page, 1)[:, :n + p].repeat_interleave(group, 0)
+        codes = torch.where(sv[..., None] > 0, v.abs() / sv.clamp_min(1e-300)[..., None], torch.zeros_like(v))
         q = x[t0:t0 + n].transpose(0, 1)
         keep = torch.ones(n, n + p, dtype=torch.bool, device=q.device)
         if causal:
@@ -117,18 +121,23 @@ def attention(cache, qkv, new, past, table, q_heads, causal, scale):
         pr = torch.softmax(s, -1)
         out[t0:t0 + n] = (pr @ v).transpose(0, 1)
         mag[t0:t0 + n] = (pr @ v.abs()).transpose(0, 1)
+        floor[t0:t0 + n] = ((pr * torch.where(sv > 0, sv, torch.ones_like(sv))[:, None]).amax(-1, keepdim=True) *
+                            (keep.double() @ codes)).transpose(0, 1)
         dot[t0:t0 + n] = ((q.abs() @ k.abs().transpose(1, 2)).amax(-1) * abs(scale)).transpose(0, 1)
         t0 += n
-    return out.reshape(T, -1), mag.reshape(T, -1), dot.repeat_interleave(hd, -1).reshape(T, -1)
+    return tuple(t.reshape(T, -1) for t in (out, mag, dot.repeat_interleave(hd, -1), floor))
 
 
-def attention_bound(out, mag, dot, hd):
+def attention_bound(out, mag, dot, floor, hd):
     """How far the bf16 output of an fp32 kernel may be from `out`: half a bf16 step of the
     result; weights off by 2^-11 (f16) + 2^-20 (exponential, running sums of them) and by what
     the logits are off, hd + 8 fp32 operations of half a step each on sum |q k| (counted whole
-    steps: the tensor cores may truncate), in numerator and denominator alike."""
+    steps: the tensor cores may truncate), in numerator and denominator alike.  f16 has no step
+    below 2^-24: a weight is held at 2^7 or more where the row's largest is, so it is off by at most
+    half of 2^-24 / 2^7 = 2^-32 of the largest, whatever its own size (a row whose largest weights
+    fall on a page of zero values shows it)."""
     ds = (hd + 8) * 2.0 ** -23 * dot
-    return 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2.0 ** -19 + 2.0 * ds) * mag * 1.01 + 1e-30
+    return 2.0 ** -8 * out.abs() + (2.0 ** -11 + 2.0 ** -19 + 2.0 * ds) * mag * 1.01 + 2.0 ** -32 * floor + 1e-30
 
 
 class Batch:

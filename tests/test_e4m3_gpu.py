@@ -268,10 +268,10 @@ def test_append_leaves_other_bytes_alone_and_reports_bad_input(cuda_dev):
 # ------------------------------------------------------------ attention over the cache
 def _attend(b, ops, cache, causal=True, scale=None, check=None):
     out = ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.max_kv, b.table, cache, b.q_heads, causal, scale)
-    want, mag, dot = ref.attention(cache, b.qkv, b.new, b.past, b.table, b.q_heads, causal,
-                                   b.hd ** -0.5 if scale is None else scale)
+    want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, b.past, b.table, b.q_heads, causal,
+                                          b.hd ** -0.5 if scale is None else scale)
     T = sum(b.new)
-    err, bound = (out[:T].double() - want).abs(), ref.attention_bound(want, mag, dot, b.hd)
+    err, bound = (out[:T].double() - want).abs(), ref.attention_bound(want, mag, dot, floor, b.hd)
     assert torch.all(err <= bound), float((err / bound).max())
     ops.device_status(0)
     return out
