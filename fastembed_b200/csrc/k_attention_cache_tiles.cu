@@ -6,10 +6,14 @@
 // A unit is (sequence, key-value head, ROWS rows), the rows being the new tokens times the
 // query heads of the group, r = token * group + head, so one pass over the cache serves every
 // query head that shares it.  A unit is one CTA: NS streams of 128 rows (two for head_dim 64
-// and 128) over the same 128-token items, each with its own S, O and softmax warpgroup, so that
-// one stream's softmax runs under the other's MMAs.  Units go out longest first (a causal
-// prompt's last tile sees the most tokens); a unit's items may be split over CTAs.
+// and 128) over the same 128-token items, each with its own S, O and softmax warpgroup.  Units go
+// out longest first (a causal prompt's last tile sees the most tokens); a unit's items may be
+// split over CTAs.
 //
+//   Steps of 64 tokens: a stream has two 64-column S slots in TMEM, S of a step goes into the
+//     slot that the step before the last has left, and so S(k + 1) and PV(k - 1) run under the
+//     softmax of step k.  (One 128-column slot per stream, where S had to wait for the previous
+//     PV, took 250 us on the case below that takes 224 us now.)
 //   K stays in 8 bits: S = Q K^T as kind::f8f6f4 with Q in two e4m3 parts, q = hi + lo.  A bf16
 //     has 8 significant bits and each part holds 4, so after a power-of-two scaling of the row
 //     (maximum in [128, 256)) the split is exact down to 2^-10 of the row's largest element and
@@ -18,21 +22,24 @@
 //   V becomes f16 (exact) on four converter warps, which also zero the slots past the
 //     sequence's end; O += P V as kind::f16 with P (f16) in TMEM over S.
 //   Scales: an item's 16-token groups (a page holds at least one) each have (sk, log2 sv,
-//     1 / sv) in a small ring that the producer fills.  P's reference moves only when a tile's
+//     1 / sv) in a small ring that the producer fills.  P's reference moves only when a step's
 //     maximum exceeds it by 2^8, so P lies below 2^15.  The sum of P / sv underflows only where
 //     the scales of a sequence's pages differ by more than 2^30: from the first such item on the
 //     exponentials of the sum are taken apart from those of P.
 //
 //   warp 0       TMA producer: K and V pages of each item (a box is a page; a page that is not
 //                there, or past the end, is read as zeros from outside the tensor)
-//   warp 1       TMEM owner and MMA issuer (an elected lane), in the fixed order
-//                PV0(n), S0(n+1), PV1(n), S1(n+1)
+//   next NS      MMA issuers, one per stream (an elected lane each): PV(k), S(k + 2).  One warp for
+//                both streams was what bounded the kernel: waits on barriers long complete, commits
+//                and issue cost a warp some 600 clocks a product beside busy softmax warps, 2,500 a
+//                step where the tensor cores need 1,290.
 //   next 4 NS    softmax (thread = row); they also quantise Q into shared memory
 //   last 4       V converters
 // Waits are bounded; on timeout the CTA records FE_ERR_DEVICE_TIMEOUT and leaves.
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fe_attention_cache.cuh"
 
@@ -54,7 +61,7 @@ struct TileCfg {
     static constexpr int RS = HD == 256 ? 1 : 2;      // raw V slots
     static constexpr int VS = HD == 256 ? 1 : 2;      // f16 V slots
     static constexpr int SOFT = 4 * NS;               // softmax warps
-    static constexpr int WARPS = 2 + SOFT + 4;
+    static constexpr int WARPS = 1 + NS + SOFT + 4;
     static constexpr int THREADS = 32 * WARPS;
     static constexpr uint32_t USED = 1024 + NS * 2 * KT + KS * KT + RS * KT + VS * VT + kEnt * 8 * 16 + 512;
     // more than half of an SM's: a CTA takes all 512 TMEM columns, a second one would wait for them
@@ -71,27 +78,37 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c)
     else return (c >> 3) * (TK * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Shared-memory descriptor of such a tile (K-major), advanced by `kk` steps of 32 bytes.
-template <int HD>
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, int kk)
-{
-    if constexpr (HD == 64) {
-        uint64_t d = sdesc_sw128(addr + 32 * kk, 16, 512);
-        d &= ~(static_cast<uint64_t>(7) << 61);
-        return d | (static_cast<uint64_t>(4) << 61);  // 64-byte swizzle
-    } else {
-        return sdesc_sw128(addr + (kk >> 2) * (TK * 128) + (kk & 3) * 32, 16, 1024);
-    }
-}
+// Shared-memory descriptors as (address + LBO, SBO + version + layout) words: bits [0,14) address
+// >> 4, [16,30) leading byte offset >> 4, [32,46) stride byte offset >> 4, [46,48) version 1,
+// [61,64) layout (2 = 128-byte swizzle, 4 = 64-byte).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | (lbo >> 4 << 16); }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo, uint32_t layout) { return (sbo >> 4) | (1u << 14) | (layout << 29); }
 
-__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate)
+// The MMAs of this kernel take their shared-memory descriptors as a low word (the address, which
+// is all that changes) and a high word fixed per layout: the issuing warp shares its scheduler
+// with softmax warps, and 64-bit address arithmetic is instructions that it waits for.
+template <uint32_t HI_A, uint32_t HI_B, bool ACC>
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %4};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(HI_A), "n"(HI_B), "n"(ACC ? 1 : 0)
+        : "memory");
+}
+
+template <uint32_t HI_B>
+__device__ __forceinline__ void umma_pv(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %4};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(HI_B), "r"(accumulate)
         : "memory");
 }
 
@@ -107,12 +124,17 @@ __host__ __device__ constexpr uint32_t idesc_f16_bt(int M, int N)
     return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// e4m3(a), e4m3(b) and what they leave: hi = e4m3(x), lo = e4m3(x - hi); NaN where x is not finite
-__device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t &hi, uint32_t &lo)
+// Two f16 values x (up to 256, 8 significant bits) as hi + lo: hi = e4m3(x), lo = e4m3(x - hi),
+// the difference exact in f16; NaN stays NaN.
+__device__ __forceinline__ void split_e4m3x2(uint32_t x, uint32_t &hi, uint32_t &lo)
 {
-    hi = cvt_e4m3x2(a, b);
-    const float2 h = e4m3x2_to_f32x2(hi);
-    lo = cvt_e4m3x2(a - h.x, b - h.y);
+    uint16_t h, l;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
+    const uint32_t back = e4m3x2_to_f16x2(h);
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&back));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(*reinterpret_cast<const uint32_t *>(&d)));
+    hi = h;
+    lo = l;
 }
 
 template <int HD>
@@ -138,13 +160,13 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     uint64_t *v_full = r_empty + RS;    // [VS] one arrival per converter warp
     uint64_t *v_empty = v_full + VS;    // [VS] a commit per stream
     uint64_t *e_full = v_empty + VS;    // [kEnt]
-    uint64_t *s_full = e_full + kEnt;   // [2]
-    uint64_t *p_full = s_full + 2;      // [2] one arrival per softmax warp
-    uint64_t *pv_done = p_full + 2;     // [2]
-    uint64_t *probe = pv_done + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(probe + 1);
+    uint64_t *s_full = e_full + kEnt;     // [NS][slot]
+    uint64_t *p_full = s_full + 2 * NS;   // [NS][slot] one arrival per softmax warp
+    uint64_t *pv_done = p_full + 2 * NS;  // [NS][slot]
+    uint64_t *probe = pv_done + 2 * NS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(probe + NS);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    static_assert((NS + 2 * KS + 2 * RS + 2 * VS + kEnt + 7) * 8 + 8 <= 512, "barrier space");
+    static_assert((8 * NS + 2 * KS + 2 * RS + 2 * VS + kEnt) * 8 + 8 <= 512, "barrier space");
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -177,12 +199,12 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
             mbar_init(&v_empty[i], NS);
         }
         for (int i = 0; i < kEnt; ++i) mbar_init(&e_full[i], 1);
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * NS; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
         }
-        mbar_init(probe, 1);
+        for (int i = 0; i < NS; ++i) mbar_init(&probe[i], 1);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_k);
@@ -196,11 +218,13 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     __syncthreads();
     tc_fence_after();
     grid_dep_launch();
-    const uint32_t tmem = *tmem_slot;  // S slots at 0 and 128, O of stream s at 256 + s * HD
+    const uint32_t tmem = *tmem_slot;  // S slot k & 1 of stream s at 128 s + 64 (k & 1), O of stream s at 256 + s * HD
 
-    // S slot and phase of item n: two streams own a slot each, one stream alternates
-    auto slot_of = [](int s, int n) { return NS == 2 ? s : n & 1; };
-    auto phase_of = [](int n) -> uint32_t { return NS == 2 ? n & 1 : (n >> 1) & 1; };
+    // step k is half k & 1 of item k / 2; a step that lies past the end is not there
+    const int steps = items == 0 ? 0 : 2 * items - (end - (j0 + items - 1) * TK <= 64 ? 1 : 0);
+    // a stream's barriers of step k: slot k & 1, in turn
+    auto slot_of = [](int s, int k) { return 2 * s + (k & 1); };
+    auto phase_of = [](int k) -> uint32_t { return (k >> 1) & 1; };
     // whole warps wait, and give up together
     auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
         if (__all_sync(0xffffffffu, mbar_wait(bar, parity))) return true;
@@ -211,9 +235,9 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
-        // K(n) goes into its slot once S(n - KS) of every stream is done, and S(m) is issued only
-        // after the softmax of item m - 1 (one stream: m - 2) has read its scales: when the scales of
-        // item n are written, those of item n - KS - 2 and before have been read, so 8 entries do.
+        // K(n) goes into its slot once every stream's S over item n - KS is done.  The second of those
+        // is issued after the PV of the step two before it, the last of item n - KS - 1, so after
+        // the softmax that read that item's scales: KS + 1 entries are in use, 8 do.
         const bool leader = elect_lane();
         const int page = 1 << a.page_log2, ppi = a.page_log2 >= 7 ? 1 : TK >> a.page_log2;  // pages per item
         const int64_t none = static_cast<int64_t>(a.pages) * a.kv_heads << a.page_log2;     // a row outside the pool
@@ -280,117 +304,177 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         // every load this warp started lands before the CTA exits
         for (int n = max(0, kn - KS); n < kn; ++n) (void)mbar_wait_drain(&k_full[n % KS], (n / KS) & 1);
         for (int n = max(0, vn - RS); n < vn; ++n) (void)mbar_wait_drain(&r_full[n % RS], (n / RS) & 1);
-    } else if (warp == 1) {
-        // ------------------------------------------------ MMA issuer
+    } else if (warp <= NS) {
+        // ------------------------------------------------ MMA issuer of a stream
+        const int s = warp - 1;
         const bool leader = elect_lane();
         constexpr uint32_t idesc_o = idesc_f16_bt(128, HD);
+        constexpr uint32_t kt = C::KT >> 4, vt = C::VT >> 4;  // in descriptor units of 16 bytes
+        constexpr uint32_t half_k = (HD == 64 ? 64 * 64 : 64 * 128) >> 4, half_v = 64 * 128 >> 4, box = TK * 128 >> 4;
+        constexpr uint32_t hi_k = HD == 64 ? desc_hi(512, 4) : desc_hi(1024, 2), hi_v = desc_hi(1024, 2);
+        auto wait_lane = [&](uint64_t *bar, uint32_t parity) -> bool {
+            if (mbar_wait(bar, parity)) return true;
+            report(status, DEV_TIMEOUT);
+            *abort_flag = 1;
+            return false;
+        };
         bool issued = false;
-        auto issue_s = [&](int s, int n) -> bool {
-            const int ks = n % KS, sl = slot_of(s, n);
-            if (!wait(&k_full[ks], (n / KS) & 1)) return false;
-            if (n == 0 && !wait(&q_full[s], 0)) return false;
-            // P of the slot's previous item consumed
-            if (n >= (NS == 2 ? 1 : 2) && !wait(&pv_done[sl], phase_of(n - (NS == 2 ? 1 : 2)))) return false;
+        const uint32_t qs = desc_lo(smem_u32(sQ) + s * 2 * C::KT, 16), kd0 = desc_lo(smem_u32(sK), 16);
+        const uint32_t vd0 = desc_lo(smem_u32(sV), TK * 128);  // MN-major: LBO between 64-column boxes
+        const uint32_t st = tmem + s * 128, od = tmem + 256 + s * HD;
+        // the K ring's position of the next S, the V ring's of the next PV
+        struct Ring {
+            uint32_t slot, phase, at;
+            __device__ __forceinline__ void next(uint32_t depth, uint32_t size)
+            {
+                ++slot;
+                at += size;
+                if (slot == depth) slot = 0, at = 0, phase ^= 1;
+            }
+        };
+        Ring kr = {}, vr = {};
+        // left: tokens from the step's first on (more than 0); par: the phase of the step's item
+        auto issue_s = [&](auto hc, bool first, uint32_t par, int left) -> bool {
+            constexpr int h = decltype(hc)::value;
+            if (h == 0 && !wait_lane(&k_full[kr.slot], kr.phase)) return false;
+            if (first) {
+                if (h == 0 && !wait_lane(&q_full[s], 0)) return false;
+            } else if (!wait_lane(&pv_done[2 * s + h], par ^ 1)) {  // P of the slot's previous step consumed
+                return false;
+            }
             tc_fence_after();
-            const int n16 = min(TK, (end - (j0 + n) * TK + 15) & ~15);
-            const uint32_t idesc = idesc_f8(128, n16);
-            const uint32_t qa = smem_u32(sQ + s * 2 * C::KT), ka = smem_u32(sK + ks * C::KT);
+            const uint32_t idesc = idesc_f8(128, min(64, (left + 15) & ~15));
+            const uint32_t kd = kd0 + kr.at + h * half_k;
+            if (leader) {
+                umma_f8<hi_k, hi_k, false>(st + 64 * h, qs, kd, idesc);
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
-#pragma unroll
-                for (int kk = 0; kk < HD / 32; ++kk)
-                    if (leader)
-                        umma_f8(tmem + sl * 128, tile_desc<HD>(qa + part * C::KT, kk), tile_desc<HD>(ka, kk), idesc,
-                                (part | kk) != 0 ? 1u : 0u);
+                for (int i = 1; i < HD / 16; ++i) {  // the steps of 32 codes of both parts of Q
+                    const int part = i / (HD / 32), kk = i % (HD / 32);
+                    const uint32_t at = HD == 64 ? 2 * kk : (kk >> 2) * box + (kk & 3) * 2;
+                    umma_f8<hi_k, hi_k, true>(st + 64 * h, qs + part * kt + at, kd + at, idesc);
+                }
+                umma_commit(&s_full[2 * s + h]);
+                if (h) umma_commit(&k_empty[kr.slot]);
+            }
+            __syncwarp();  // no lane goes on to wait before the leader has issued
             issued = true;
-            if (leader) {
-                umma_commit(&s_full[sl]);
-                umma_commit(&k_empty[ks]);
-            }
+            if (h) kr.next(KS, kt);
             return true;
         };
-        auto issue_pv = [&](int s, int n) -> bool {
-            const int vs = n % VS, sl = slot_of(s, n);
-            if (!wait(&p_full[sl], phase_of(n))) return false;
-            if (!wait(&v_full[vs], (n / VS) & 1)) return false;
+        auto issue_pv = [&](auto hc, bool first, uint32_t par, int left) -> bool {
+            constexpr int h = decltype(hc)::value;
+            if (h == 0 && !wait_lane(&v_full[vr.slot], vr.phase)) return false;
+            if (!wait_lane(&p_full[2 * s + h], par)) return false;
             tc_fence_after();
-            const int steps = (min(TK, end - (j0 + n) * TK) + 15) >> 4;
-            const uint64_t vd = sdesc_sw128(smem_u32(sV + vs * C::VT), TK * 128, 1024);
-            for (int k = 0; k < steps; ++k)  // 16 tokens = 16 rows of 128 bytes
-                if (leader)
-                    umma_f16_ts(tmem + 256 + s * HD, tmem + sl * 128 + k * 8, vd + static_cast<uint64_t>(k * 128), idesc_o,
-                                (n | k) != 0 ? 1u : 0u);
+            const uint32_t vd = vd0 + vr.at + h * half_v, pt = st + 64 * h;  // 16 tokens = 16 rows of 128 bytes
             if (leader) {
-                umma_commit(&pv_done[sl]);
-                umma_commit(&v_empty[vs]);
+                umma_pv<hi_v>(od, pt, vd, idesc_o, h == 0 && first ? 0u : 1u);
+                if (left > 48) {
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) umma_pv<hi_v>(od, pt + 8 * i, vd + i * 128, idesc_o, 1u);
+                } else {
+                    for (int i = 1; 16 * i < left; ++i) umma_pv<hi_v>(od, pt + 8 * i, vd + i * 128, idesc_o, 1u);
+                }
+                umma_commit(&pv_done[2 * s + h]);
+                if (h) umma_commit(&v_empty[vr.slot]);
             }
+            __syncwarp();
+            if (h) vr.next(VS, vt);
             return true;
         };
-        bool ok = items > 0;
-        for (int s = 0; s < NS && ok; ++s) ok = issue_s(s, 0);
-        for (int n = 0; n < items && ok && !*abort_flag; ++n) {
-            const bool more = n + 1 < items;
-            if constexpr (NS == 2)
-                ok = issue_pv(0, n) && (!more || issue_s(0, n + 1)) && issue_pv(1, n) && (!more || issue_s(1, n + 1));
-            else  // the next S fills the other slot while this item's softmax runs
-                ok = (!more || issue_s(0, n + 1)) && issue_pv(0, n);
+        constexpr std::integral_constant<int, 0> c0{};
+        constexpr std::integral_constant<int, 1> c1{};
+        int left = min(end - j0 * TK, items * TK);  // tokens of this CTA's part from this item's first on
+        uint32_t par = 0;
+        bool ok = items > 0 && issue_s(c0, true, 0, left) && (left <= 64 || issue_s(c1, true, 0, left - 64));
+        for (int n = 0; n < items && ok && !*abort_flag; ++n, left -= TK, par ^= 1) {
+            const bool first = n == 0;
+            ok = issue_pv(c0, first, par, left) && (left <= TK || issue_s(c0, false, par ^ 1, left - TK));
+            if (left > 64)
+                ok = ok && issue_pv(c1, first, par, left - 64) &&
+                     (left <= TK + 64 || issue_s(c1, false, par ^ 1, left - TK - 64));
         }
         if (issued) {  // MMAs retire before TMEM is released
-            if (leader) umma_commit(probe);
-            (void)mbar_wait_drain(probe, 0);
+            if (leader) umma_commit(&probe[s]);
+            (void)mbar_wait_drain(&probe[s], 0);
         }
-    } else if (warp < 2 + C::SOFT) {
+    } else if (warp <= NS + C::SOFT) {
         // ------------------------------------------------ softmax: thread = row
-        const int s = (warp - 2) >> 2, q = warp & 3;
+        const int s = (warp - 1 - NS) >> 2, q = warp & 3;
         const int r = q * 32 + lane;  // row within the stream == TMEM lane
         const int rr = r0 + 128 * s + r;
         const bool live = rr < rows, warp_live = r0 + 128 * s + q * 32 < rows;
         const int token = live ? rr / a.group : 0, head = kvh * a.group + (live ? rr - token * a.group : 0);
         const int vis = !live ? 0 : a.causal ? sq.past + token + 1 : sq.kv;  // tokens this row sees
+        bool ok = true;
         float qf = 0.f;
         {
-            // Q: the row's maximum to [128, 256), split in two e4m3 parts
-            const __nv_bfloat16 *p = a.qkv + (sq.t0 + token) * a.row + static_cast<int64_t>(head) * HD;
-            uint32_t m = 0;  // of |q| as bf16 bits: their order is that of the values
-            if (live)
-#pragma unroll 4
-                for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(p + 8 * c);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t x = w[i] & 0x7fffu, y = (w[i] >> 16) & 0x7fffu;
-                        m = max(m, max(x < 0x7f80u ? x : 0u, y < 0x7f80u ? y : 0u));
-                    }
-                }
-            int e = static_cast<int>(m >> 7) - 127 - 7;  // q * 2^-e has its maximum in [128, 256)
-            e = max(-100, e);
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-            // a negative softmax scale turns Q's signs, so that the logit factor is never negative
-            const float sign = a.scale_log2 < 0.f ? -down : down;
-            qf = fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            // Q: the row's maximum to [128, 256), split in two e4m3 parts.  HD / 16 lanes share a row (16
+            // values each), RPI rows at a time, the loads of up to eight such rounds in flight together.
+            constexpr int LPR = HD / 16, RPI = 32 / LPR, IT = 32 / RPI < 8 ? 32 / RPI : 8;
+            const int c = lane % LPR;
+            const int row0 = q * 32 + lane / LPR;  // of this lane in the first round, within the stream
+            const int first = r0 + 128 * s + row0;
+            int tk = first / a.group, hd = first - tk * a.group;  // of the round's row; RPI rows on each round
+            const int tk_up = RPI / a.group, hd_up = RPI - tk_up * a.group;
             uint8_t *hi = sQ + s * 2 * C::KT, *lo = hi + C::KT;
-#pragma unroll 2
-            for (int c = 0; c < HD / 16; ++c) {
-                uint4 u[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                if (live) {
-                    u[0] = *reinterpret_cast<const uint4 *>(p + 16 * c);
-                    u[1] = *reinterpret_cast<const uint4 *>(p + 16 * c + 8);
-                }
-                const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-                uint32_t h[4], l[4];
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32 / RPI; i0 += IT) {
+                uint4 u[IT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x = unpack_bf16x2(w[2 * i]), y = unpack_bf16x2(w[2 * i + 1]);
-                    uint32_t h0, l0, h1, l1;
-                    split_e4m3x2(scaled_or_nan(x.x, sign), scaled_or_nan(x.y, sign), h0, l0);
-                    split_e4m3x2(scaled_or_nan(y.x, sign), scaled_or_nan(y.y, sign), h1, l1);
-                    h[i] = h0 | (h1 << 16);
-                    l[i] = l0 | (l1 << 16);
+                for (int i = 0; i < IT; ++i) {
+                    u[i][0] = u[i][1] = make_uint4(0, 0, 0, 0);
+                    if (first + (i0 + i) * RPI < rows) {
+                        const __nv_bfloat16 *p =
+                            a.qkv + (sq.t0 + tk) * a.row + static_cast<int64_t>(kvh * a.group + hd) * HD + 16 * c;
+                        u[i][0] = *reinterpret_cast<const uint4 *>(p);
+                        u[i][1] = *reinterpret_cast<const uint4 *>(p + 8);
+                    }
+                    tk += tk_up;
+                    hd += hd_up;
+                    if (hd >= a.group) hd -= a.group, ++tk;
                 }
-                const uint32_t at = tile_offset<HD>(r, c);
-                *reinterpret_cast<uint4 *>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+                for (int i = 0; i < IT; ++i) {
+                    uint32_t w[8] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w, u[i][1].x, u[i][1].y, u[i][1].z, u[i][1].w};
+                    uint32_t m2 = 0;  // of |q| as bf16 bits, both halves: their order is that of the values
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) m2 = __vmaxu2(m2, w[j] & 0x7fff7fffu);
+                    uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+#pragma unroll
+                    for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+                    if (__any_sync(0xffffffffu, m >= 0x7f80u)) {  // infinities and NaN: as NaN, the maximum without them
+                        m = 0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if ((w[j] & 0x7f80u) == 0x7f80u) w[j] |= 0x7fffu;
+                            else m = max(m, w[j] & 0x7fffu);
+                            if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] |= 0x7fff0000u;
+                            else m = max(m, (w[j] >> 16) & 0x7fffu);
+                        }
+#pragma unroll
+                        for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+                    }
+                    const int e = max(-100, static_cast<int>(m >> 7) - 127 - 7);  // q 2^-e has its maximum in [128, 256)
+                    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    // a negative softmax scale turns Q's signs, so that the logit factor is never negative
+                    const float sign = a.scale_log2 < 0.f ? -down : down;
+                    const int mine = __shfl_sync(0xffffffffu, e, lane % RPI * LPR);  // row (i0 + i) RPI + lane % RPI
+                    if (lane / RPI == i0 + i)
+                        qf = fabsf(a.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 + mine) << 23);
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 x = unpack_bf16x2(w[j]);
+                        uint32_t h2, l2;
+                        split_e4m3x2(pack_f16x2(x.x * sign, x.y * sign), h2, l2);
+                        h[j >> 1] = j & 1 ? h[j >> 1] | (h2 << 16) : h2;
+                        l[j >> 1] = j & 1 ? l[j >> 1] | (l2 << 16) : l2;
+                    }
+                    const uint32_t at = tile_offset<HD>(row0 + (i0 + i) * RPI, c);
+                    *reinterpret_cast<uint4 *>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -399,96 +483,86 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
         const uint32_t tO = tmem + lanes + 256 + s * HD;
         float m_run = -INFINITY, l_run = 0.f;
-        bool ok = true;
-        for (int n = 0; n < items; ++n) {
-            const int sl = slot_of(s, n);
-            const uint32_t tS = tmem + lanes + sl * 128;
-            if (!(ok = wait(&e_full[n % kEnt], (n / kEnt) & 1) && wait(&s_full[sl], phase_of(n)))) break;
+        for (int k = 0; k < steps && ok; ++k) {  // 64 tokens at a time, from registers
+            const int n = k >> 1, h = k & 1, c0 = 64 * h;
+            const uint32_t tS = tmem + lanes + s * 128 + 64 * h;
+            if (h == 0 && !(ok = wait(&e_full[n % kEnt], (n / kEnt) & 1))) break;
+            if (!(ok = wait(&s_full[slot_of(s, k)], phase_of(k)))) break;
             tc_fence_after();
-            const float4 *en = ent + (n % kEnt) * 8;
-            const int base = (j0 + n) * TK, cols = min(TK, end - base), lim = vis - base;
+            const float4 *en = ent + (n % kEnt) * 8 + (c0 >> 4);
+            const int lim = vis - (j0 + n) * TK - c0;  // columns of the step that the row sees
+            const bool spread = ent[(n % kEnt) * 8].w != 0.f;
             float alpha = 1.f;
             if (warp_live) {
-                const bool spread = en[0].w != 0.f;
-                float top = m_run;
-                for (int c = 0; c < cols; c += 32) {
-                    uint32_t v[32];
-                    __syncwarp();
-                    tmem_ld_x32(tS + c, v);
-                    tmem_wait_ld_regs(v);
+                uint32_t v[64];
+                tmem_ld_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(v));
+                tmem_ld_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v));
+                tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                if (!__all_sync(0xffffffffu, 64 <= lim)) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float m0 = -INFINITY, m1 = -INFINITY;
-                        if (c + 32 <= lim) {  // nothing masked
-#pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                m0 = max3f(m0, __uint_as_float(v[16 * h + i]), __uint_as_float(v[16 * h + i + 1]));
-                                m1 = max3f(m1, __uint_as_float(v[16 * h + i + 2]), __uint_as_float(v[16 * h + i + 3]));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (c + 16 * h + i < lim) m0 = fmaxf(m0, __uint_as_float(v[16 * h + i]));
-                        }
-                        m0 = fmaxf(m0, m1);
-                        const float4 e = en[(c >> 4) + h];
-                        if (m0 != -INFINITY) top = fmaxf(top, fmaf(m0, qf * e.x, e.y));
-                    }
+                    for (int i = 0; i < 64; ++i)
+                        if (i >= lim) v[i] = 0xff800000u;  // -inf
                 }
-                // the reference rises only when a tile exceeds it by more than 2^8
+                float top = -INFINITY, f[4], g[4], z[4];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    const float4 e = en[i4];
+                    // never 0, so that masked logits stay -inf (page scales of 0 have codes of 0)
+                    f[i4] = fmaxf(qf * e.x, 1e-30f);
+                    g[i4] = e.y;
+                    z[i4] = e.z;
+                    const uint32_t *w = v + 16 * i4;
+                    float m0 = __uint_as_float(w[0]), m1 = __uint_as_float(w[1]);
+#pragma unroll
+                    for (int i = 2; i < 14; i += 4) {
+                        m0 = max3f(m0, __uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+                        m1 = max3f(m1, __uint_as_float(w[i + 2]), __uint_as_float(w[i + 3]));
+                    }
+                    m0 = max3f(m0, __uint_as_float(w[14]), __uint_as_float(w[15]));
+                    top = fmaxf(top, fmaf(fmaxf(m0, m1), f[i4], g[i4]));
+                }
+                // the reference rises only when a step exceeds it by more than 2^8
                 if (top > m_run + kLazy || m_run == -INFINITY) {
+                    top = fmaxf(top, m_run);
                     alpha = m_run == -INFINITY ? 0.f : exp2_fast(m_run - top);
                     m_run = top;
                 }
                 const float shift = m_run == -INFINITY ? 0.f : kBoost - m_run;
                 float sum = 0.f;
-                __syncwarp();
-                for (int c = 0; c < cols; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld_x32(tS + c, v);
-                    tmem_wait_ld_regs(v);
-                    uint32_t pk[16];
+                if (spread) {  // the sum's terms P / sv from their own exponentials
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 e = en[(c >> 4) + h];
-                        const float f = qf * e.x, g = e.y + shift;
-                        float s0 = 0.f, s1 = 0.f;
-                        if (c + 16 * h >= lim) {  // all masked
+                    for (int i4 = 0; i4 < 4; ++i4)
+                        if (z[i4] != 0.f)
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) pk[8 * h + i] = 0;
-                            continue;
-                        }
-                        const bool whole = c + 16 * h + 16 <= lim;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float p0, p1;
-                            fma_f32x2(p0, p1, __uint_as_float(v[16 * h + 2 * i]), __uint_as_float(v[16 * h + 2 * i + 1]), f, g);
-                            p0 = exp2_fast(p0);
-                            p1 = exp2_fast(p1);
-                            if (!whole) {
-                                if (c + 16 * h + 2 * i >= lim) p0 = 0.f;
-                                if (c + 16 * h + 2 * i + 1 >= lim) p1 = 0.f;
-                            }
-                            add_f32x2(s0, s1, p0, p1);
-                            pk[8 * h + i] = pack_f16x2(p0, p1);
-                        }
-                        if (!spread) {
-                            sum = fmaf(s0 + s1, e.z, sum);
-                        } else if (e.z != 0.f) {  // P / sv from its own exponentials
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (c + 16 * h + i < lim) sum += exp2_fast(fmaf(__uint_as_float(v[16 * h + i]), f, shift));
-                        }
-                    }
-                    __syncwarp();
-                    tmem_st_x16(tS + (c >> 1), pk);
+                            for (int i = 0; i < 16; ++i) sum += exp2_fast(fmaf(__uint_as_float(v[16 * i4 + i]), f[i4], shift));
                 }
+                uint32_t pk[32];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4) {
+                    const uint32_t *w = v + 16 * i4;
+                    const float gk = g[i4] + shift;
+                    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float p0, p1;
+                        fma_f32x2(p0, p1, __uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]), f[i4], gk);
+                        p0 = exp2_fast(p0);
+                        p1 = exp2_fast(p1);
+                        add_f32x2(s0, s1, p0, p1);
+                        pk[8 * i4 + i] = pack_f16x2(p0, p1);
+                    }
+                    if (!spread) sum = fmaf(s0 + s1, z[i4], sum);
+                }
+                __syncwarp();
+                tmem_st_x32(tS, pk);
                 l_run = fmaf(l_run, alpha, sum);
                 tmem_wait_st();
             }
-            // O *= alpha after the previous item's PV and before this one's
-            if (n > 0 && warp_live && __any_sync(0xffffffffu, alpha != 1.f)) {
-                if (!(ok = wait(&pv_done[slot_of(s, n - 1)], phase_of(n - 1)))) break;
+            // O *= alpha after the previous step's PV and before this one's
+            const bool rescale = k > 0 && warp_live && __any_sync(0xffffffffu, alpha != 1.f);
+            if (rescale) {
+                if (!(ok = wait(&pv_done[slot_of(s, k - 1)], phase_of(k - 1)))) break;
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
@@ -503,9 +577,9 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[sl]);
+            if (lane == 0) mbar_arrive(&p_full[slot_of(s, k)]);
         }
-        if (ok && items > 0) ok = wait(&pv_done[slot_of(s, items - 1)], phase_of(items - 1));
+        if (ok && steps > 0) ok = wait(&pv_done[slot_of(s, steps - 1)], phase_of(steps - 1));
         tc_fence_after();
         if (ok && warp_live) {
             const int64_t orow = (static_cast<int64_t>(sq.t0) + token) * a.q_heads + head;
@@ -542,7 +616,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         }
     } else {
         // ------------------------------------------------ V converters
-        const int t = threadIdx.x - 32 * (2 + C::SOFT);
+        const int t = threadIdx.x - 32 * (1 + NS + C::SOFT);
         constexpr int CPR = HD / 16;  // 16-code chunks per row
         for (int n = 0; n < items && !*abort_flag; ++n) {
             const int rs = n % RS, vs = n % VS;
