@@ -23,57 +23,72 @@
 namespace fe {
 namespace {
 
-// max |v| of 8 bf16 as the bits of an fp32 value, non-finite ones left out; bad: any of those
-__device__ __forceinline__ float amax8(const uint4 &u, bool &bad)
+// The largest |v| of 8 bf16 as bf16 bits: they order like the values, infinities and NaN (0x7f80
+// and above) last.
+constexpr uint32_t kBf16Inf = 0x7f80u;
+__device__ __forceinline__ uint32_t amax8(const uint4 &u)
 {
-    float m = 0.f;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack_bf16x2(w[i]);
-        bad |= !(fabsf(f.x) <= 3.402823466e38f) || !(fabsf(f.y) <= 3.402823466e38f);
-        m = fmaxf(m, fmaxf(finite_abs(f.x), finite_abs(f.y)));
-    }
-    return m;
+    const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
 }
 
-// The smallest power of two 2^e with amax <= 448 * 2^e, e >= kMinScaleExp; 0 for amax = 0.
-// amax widened from bf16 is 1.f * 2^E or subnormal (far below the smallest scale).
-constexpr int kMinScaleExp = -80;
-__device__ __forceinline__ float block_scale(float amax)
-{
-    if (amax == 0.f) return 0.f;
-    const uint32_t b = __float_as_uint(amax);
-    int e = static_cast<int>(b >> 23) - 127 - 8;                  // 448 = 1.75 * 2^8
-    if ((b & 0x7fffffu) > 0x600000u) ++e;                         // mantissa above 1.75
-    e = e < kMinScaleExp ? kMinScaleExp : e;
-    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-}
-
-__device__ __forceinline__ uint2 encode8(const uint4 &u, float inv, bool nan_all)
-{
-    if (nan_all) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-    return make_uint2(pack_e4m3x4(a.x * inv, a.y * inv, b.x * inv, b.y * inv),
-                      pack_e4m3x4(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
-}
-
-// zeros in place of non-finite elements (values of a poisoned token)
+// zeros in place of non-finite elements
 __device__ __forceinline__ uint4 finite_only(uint4 u)
 {
     uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
-        if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0x0000ffffu;
+        if ((w[i] & kBf16Inf) == kBf16Inf) w[i] &= 0xffff0000u;
+        if ((w[i] & (kBf16Inf << 16)) == kBf16Inf << 16) w[i] &= 0x0000ffffu;
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The smallest power of two 2^e with amax <= 448 * 2^e, e >= kMinScaleExp; 0 for amax = 0.
+// amax comes as bf16 bits (1.f * 2^E, or subnormal, far below the smallest scale); 448 = 1.75 * 2^8.
+constexpr int kMinScaleExp = -80;
+__device__ __forceinline__ float block_scale(uint32_t amax)
+{
+    if (amax == 0) return 0.f;
+    const int e = static_cast<int>(amax >> 7) - 127 - 8 + ((amax & 0x7fu) > 0x60u ? 1 : 0);  // mantissa above 1.75
+    return __uint_as_float(static_cast<uint32_t>(max(e, kMinScaleExp) + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t encode4(uint32_t x, uint32_t y, float inv)
+{
+    float2 a = unpack_bf16x2(x), b = unpack_bf16x2(y);
+    mul_f32x2(a.x, a.y, inv, inv);
+    mul_f32x2(b.x, b.y, inv, inv);
+    return pack_e4m3x4(a.x, a.y, b.x, b.y);
+}
+
+__device__ __forceinline__ uint2 encode8(const uint4 &u, float inv)
+{
+    return make_uint2(encode4(u.x, u.y, inv), encode4(u.z, u.w, inv));
 }
 
 __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float ratio)
 {
     const float2 a = e4m3x2_to_f32x2(codes & 0xffffu), b = e4m3x2_to_f32x2(codes >> 16);
     return pack_e4m3x4(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
+}
+
+// The block's largest k and v (every thread gets both).
+template <int WARPS>
+__device__ __forceinline__ void block_max(uint32_t &k, uint32_t &v, uint32_t (&red)[2][WARPS])
+{
+    k = __reduce_max_sync(0xffffffffu, k);
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) {
+        red[0][threadIdx.x >> 5] = k;
+        red[1][threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        k = max(k, red[0][i]);
+        v = max(v, red[1][i]);
+    }
 }
 
 struct AppendArgs {
@@ -90,7 +105,7 @@ template <int HD, int CH, int THREADS>
 __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int reach, int *status)
 {
     constexpr int LPT = HD / 8;  // lanes of a token: 8, 16 or 32, aligned within a warp
-    __shared__ float red[2][THREADS / 32];
+    __shared__ uint32_t red[2][2][THREADS / 32];
     const int b = blockIdx.x / reach, nth = blockIdx.x % reach, head = blockIdx.y;
     grid_dep_wait();
     grid_dep_launch();
@@ -105,20 +120,11 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
     const int64_t base = ordinal * a.page;  // first token of the page
     if (base >= end) return;
     if (nth == reach - 1 && base + a.page < end && threadIdx.x == 0) report(status, DEV_BAD_INPUT);  // longer than max_len
-    const int id = ordinal < a.width ? a.table[static_cast<int64_t>(b) * a.width + ordinal] : -1;
-    if (id < 0 || id >= a.pages) {
-        if (threadIdx.x == 0) report(status, DEV_BAD_INPUT);
-        return;
-    }
-    const int lo = past > base ? static_cast<int>(past - base) : 0;                       // first new slot
-    const int hi = end - base < a.page ? static_cast<int>(end - base) : a.page;           // past the last
-    const int64_t block = (static_cast<int64_t>(id) * a.kv_heads + head) * a.page * HD;  // codes of this (page, head)
-    const int64_t si = static_cast<int64_t>(id) * a.kv_heads + head;
-    const float k_old = lo > 0 ? a.ks[si] : 0.f, v_old = lo > 0 ? a.vs[si] : 0.f;
+    const int lo = past > base ? static_cast<int>(past - base) : 0;              // first new slot
+    const int hi = end - base < a.page ? static_cast<int>(end - base) : a.page;  // past the last
 
+    // the rows are on their way before the page is looked up
     uint4 kr[CH], vr[CH];
-    float km = 0.f, vm = 0.f;
-    uint32_t poisoned = 0;  // bit c: this thread's token of chunk c holds something non-finite
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int chunk = c * THREADS + threadIdx.x, slot = chunk / LPT, col = chunk % LPT * 8;
@@ -129,27 +135,36 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
             vr[c] = *reinterpret_cast<const uint4 *>(p + a.v_col0);
         }
     }
+    const int id = ordinal < a.width ? a.table[static_cast<int64_t>(b) * a.width + ordinal] : -1;
+    if (id < 0 || id >= a.pages) {
+        if (threadIdx.x == 0) report(status, DEV_BAD_INPUT);
+        return;
+    }
+    const int64_t si = static_cast<int64_t>(id) * a.kv_heads + head;
+    const int64_t block = si * a.page * HD;  // codes of this (page, head)
+    const float k_old = lo > 0 ? a.ks[si] : 0.f, v_old = lo > 0 ? a.vs[si] : 0.f;
+
+    uint32_t km = 0, vm = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-        bool bad = false;
-        const float mk = amax8(kr[c], bad);
-        vm = fmaxf(vm, amax8(vr[c], bad));
-        const uint32_t any = __ballot_sync(0xffffffffu, bad);
-        const uint32_t group = (LPT == 32 ? 0xffffffffu : ((1u << LPT) - 1u) << ((threadIdx.x & 31) / LPT * LPT));
-        if (any & group) poisoned |= 1u << c;
-        else km = fmaxf(km, mk);  // a poisoned token's key is stored as NaN and sets no scale
+        km = max(km, amax8(kr[c]));
+        vm = max(vm, amax8(vr[c]));
     }
-    km = warp_max(km);
-    vm = warp_max(vm);
-    if ((threadIdx.x & 31) == 0) {
-        red[0][threadIdx.x >> 5] = km;
-        red[1][threadIdx.x >> 5] = vm;
-    }
-    __syncthreads();  // also: every thread has read the old scales
+    block_max<THREADS / 32>(km, vm, red[0]);  // its barrier: every thread has read the old scales
+    uint32_t poisoned = 0;                    // bit c: this thread's token of chunk c holds something non-finite
+    if (max(km, vm) >= kBf16Inf) {            // rare: find those tokens, and the maxima without them
+        km = vm = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) {
-        km = fmaxf(km, red[0][i]);
-        vm = fmaxf(vm, red[1][i]);
+        for (int c = 0; c < CH; ++c) {
+            const uint32_t mk = amax8(kr[c]);
+            const uint32_t any = __ballot_sync(0xffffffffu, max(mk, amax8(vr[c])) >= kBf16Inf);
+            const uint32_t group = LPT == 32 ? 0xffffffffu : ((1u << (LPT & 31)) - 1u) << ((threadIdx.x & 31) / LPT * LPT);
+            if (any & group) poisoned |= 1u << c;
+            else km = max(km, mk);  // a poisoned token's key is stored as NaN and sets no scale
+            vr[c] = finite_only(vr[c]);
+            vm = max(vm, amax8(vr[c]));
+        }
+        block_max<THREADS / 32>(km, vm, red[1]);
     }
     const float k_new = fmaxf(k_old, block_scale(km)), v_new = fmaxf(v_old, block_scale(vm));
     const float k_inv = k_new > 0.f ? 1.0f / k_new : 0.f, v_inv = v_new > 0.f ? 1.0f / v_new : 0.f;
@@ -161,9 +176,9 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
     for (int c = 0; c < CH; ++c) {
         const int chunk = c * THREADS + threadIdx.x, slot = chunk / LPT;
         if (slot >= lo && slot < hi) {
-            const bool nan = (poisoned >> c) & 1u;
-            *reinterpret_cast<uint2 *>(a.k + block + chunk * 8) = encode8(kr[c], k_inv, nan);
-            *reinterpret_cast<uint2 *>(a.v + block + chunk * 8) = encode8(nan ? finite_only(vr[c]) : vr[c], v_inv, false);
+            *reinterpret_cast<uint2 *>(a.k + block + chunk * 8) =
+                (poisoned >> c) & 1u ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : encode8(kr[c], k_inv);
+            *reinterpret_cast<uint2 *>(a.v + block + chunk * 8) = encode8(vr[c], v_inv);
         }
     }
     // older tokens of the page follow a scale that grew

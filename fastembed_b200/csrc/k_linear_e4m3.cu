@@ -67,46 +67,44 @@ struct EpiArgs {
     const float *sx;        // [M]
     const float *sw;        // [N]
     const float *bias;      // [N] or null
-    const float *residual;  // [M, N] or null
     int epi;
 };
 
-// v[j] *= p[j] (or v[j] += p[j]) over W columns from col0, of which the last may lie past N
-template <int W, bool MUL>
-__device__ __forceinline__ void apply_cols(float (&v)[W], const float *__restrict__ p, int col0, int N)
+// 32 values of a column vector from col0 on, 0 past N (a multiple of 8)
+__device__ __forceinline__ void load_cols(float4 (&v)[8], const float *__restrict__ p, int col0, int N)
 {
-    if (col0 + W <= N) {
 #pragma unroll
-        for (int j = 0; j < W; j += 4) {
-            const float4 b = __ldg(reinterpret_cast<const float4 *>(p + col0 + j));
-            if constexpr (MUL) {
-                mul_f32x2(v[j], v[j + 1], b.x, b.y);
-                mul_f32x2(v[j + 2], v[j + 3], b.z, b.w);
-            } else {
-                add_f32x2(v[j], v[j + 1], b.x, b.y);
-                add_f32x2(v[j + 2], v[j + 3], b.z, b.w);
-            }
-        }
-    } else {
+    for (int j = 0; j < 8; ++j)
+        v[j] = col0 + 4 * j < N ? __ldg(reinterpret_cast<const float4 *>(p + col0 + 4 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// z_j = acc_j * (sx_i sw_j) + b_j for 32 accumulator columns
+__device__ __forceinline__ void scale_bias(float (&z)[32], const uint32_t (&u)[32], float sx, const float4 (&sw)[8],
+                                           const float4 (&b)[8])
+{
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-            if (col0 + j < N) v[j] = MUL ? v[j] * __ldg(p + col0 + j) : v[j] + __ldg(p + col0 + j);
+    for (int j = 0; j < 8; ++j) {
+        float s0 = sw[j].x, s1 = sw[j].y, s2 = sw[j].z, s3 = sw[j].w;
+        mul_f32x2(s0, s1, sx, sx);
+        mul_f32x2(s2, s3, sx, sx);
+        fma_f32x2v(z[4 * j], z[4 * j + 1], __uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), s0, s1, b[j].x, b[j].y);
+        fma_f32x2v(z[4 * j + 2], z[4 * j + 3], __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]), s2, s3, b[j].z,
+                   b[j].w);
     }
 }
 
-// 32 accumulator columns of this thread's row, scaled: acc * sx_i * sw_j
-__device__ __forceinline__ void load_scaled(uint32_t taddr, float (&v)[32], const EpiArgs &ea, float sx, int col0, int N)
+__device__ __forceinline__ void activate(float (&z)[32], int epi)
 {
-    uint32_t u[32];
-    tmem_ld_x32(taddr, u);
-    tmem_wait_ld_regs(u);
+    if (epi == E_GELU) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        v[j] = __uint_as_float(u[j]);
-        v[j + 1] = __uint_as_float(u[j + 1]);
-        mul_f32x2(v[j], v[j + 1], sx, sx);
+        for (int j = 0; j < 32; j += 2) gelu_tanh_fast2(z[j], z[j + 1]);
+    } else if (epi == E_SWISH) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) silu_fast2(z[j], z[j + 1]);
+    } else if (epi == E_RELU) {  // as a comparison: NaN stays NaN
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = z[j] < 0.f ? 0.f : z[j];
     }
-    apply_cols<32, true>(v, ea.sw, col0, N);
 }
 
 __device__ __forceinline__ uint4 pack8(const float *f)
@@ -114,82 +112,214 @@ __device__ __forceinline__ uint4 pack8(const float *f)
     return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// Drains COLS columns of one warp's 32 accumulator rows: 32-row x 128-byte slabs (two per
-// warp) staged in 128B-swizzled shared memory and stored by TMA, which clips rows >= M and
-// columns >= N.  `row` is this thread's output row, `store_row` the warp's first.
+// 32 finished columns of this thread's row into its slab row: 16-byte chunks from `first` on
+template <bool OUT_BF16>
+__device__ __forceinline__ void to_slab(uint8_t *slab, const float (&z)[32], int first, int lane)
+{
+    uint8_t *rowp = slab + lane * 128;
+#pragma unroll
+    for (int u = 0; u < (OUT_BF16 ? 4 : 8); ++u) {
+        uint4 w;
+        if constexpr (OUT_BF16) w = pack8(z + 8 * u);
+        else w = make_uint4(__float_as_uint(z[4 * u]), __float_as_uint(z[4 * u + 1]), __float_as_uint(z[4 * u + 2]),
+                            __float_as_uint(z[4 * u + 3]));
+        *reinterpret_cast<uint4 *>(rowp + (((first + u) ^ (lane & 7)) << 4)) = w;
+    }
+}
+
+// What an epilogue warp carries from tile to tile: its two 32-row x 128-byte slabs (128B-swizzled)
+// and, for the residual, a barrier each whose phase is the parity bit of `phase`.
+struct Slabs {
+    uint8_t *buf;
+    uint64_t *bar;
+    uint32_t phase, armed;
+    int pp;
+};
+
+__device__ __forceinline__ void store_slab(const CUtensorMap *tm_y, Slabs &sl, int x, int y, int lane)
+{
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_2d(tm_y, sl.buf + sl.pp * kSlab, x, y);
+        bulk_commit();
+    }
+    sl.pp ^= 1;
+}
+
+// Drains COLS columns of one warp's 32 accumulator rows; rows >= M and columns >= N are clipped
+// by the tensor map.  The next 32 columns' TMEM load and this 32's column vectors are in flight
+// before the arithmetic that needs them: with loads issued where they were used (and three
+// operations in place of two for scale and bias), gelu at 26,508 x 4,096 x 1,024 took 124 us,
+// now GELU_US; the mainloop alone needs 67.
 template <int COLS, bool OUT_BF16>
-__device__ __forceinline__ void drain(uint32_t t_row, int row, int store_row, int n0, int M, int N, const EpiArgs &ea,
-                                      float sx, const CUtensorMap *tm_y, uint8_t *bufs, int &pp, int lane)
+__device__ __forceinline__ void drain(uint32_t t_row, int store_row, int n0, int N, const EpiArgs &ea, float sx,
+                                      const CUtensorMap *tm_y, Slabs &sl, int lane)
 {
     const int epi = ea.epi;
-    constexpr int CHUNK = OUT_BF16 ? 64 : 32;  // y columns per slab
-    const bool glu = OUT_BF16 && COLS >= 128 && epi >= E_SWIGLU;
-    const int step = glu ? 2 * CHUNK : CHUNK;  // accumulator columns per slab
-#pragma unroll 1
-    for (int c = 0; c < COLS; c += step) {
-        float f[CHUNK];
-        if constexpr (OUT_BF16) {
+    uint32_t u[2][32];
+    tmem_ld_x32(t_row, u[0]);
+#pragma unroll 2
+    for (int c = 0; c < COLS; c += 32) {
+        uint32_t(&v)[32] = u[(c >> 5) & 1];
+        float4 sw[8], b[8];
+        load_cols(sw, ea.sw, n0 + c, N);
+        if (epi != E_NONE) load_cols(b, ea.bias, n0 + c, N);
+        else
 #pragma unroll
-            for (int hb = 0; hb < 2; ++hb) {
-                float v[32];
-                if (glu) {  // 32 gate columns, then their 32 inputs
-                    float u[32];
-                    const int a = c + 64 * hb;
-                    load_scaled(t_row + a, v, ea, sx, n0 + a, N);
-                    load_scaled(t_row + a + 32, u, ea, sx, n0 + a + 32, N);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        if (epi == E_SWIGLU) silu_fast2(v[j], v[j + 1]);
-                        else gelu_tanh_fast2(v[j], v[j + 1]);
-                        mul_f32x2(v[j], v[j + 1], u[j], u[j + 1]);
-                    }
-                } else {
-                    const int col0 = n0 + c + 32 * hb;
-                    load_scaled(t_row + c + 32 * hb, v, ea, sx, col0, N);
-                    if (epi != E_NONE) apply_cols<32, false>(v, ea.bias, col0, N);
-                    if (epi == E_GELU) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) gelu_tanh_fast2(v[j], v[j + 1]);
-                    } else if (epi == E_SWISH) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) silu_fast2(v[j], v[j + 1]);
-                    } else if (epi == E_RELU) {  // as a comparison: NaN stays NaN
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 32; ++j) f[32 * hb + j] = v[j];
-            }
-        } else {
-            const int col0 = n0 + c;
-            load_scaled(t_row + c, f, ea, sx, col0, N);
-            if (epi != E_NONE) apply_cols<32, false>(f, ea.bias, col0, N);
-            if (epi == E_RESID && row < M) {
-                const float *rp = ea.residual + static_cast<size_t>(row) * N;
-                apply_cols<32, false>(f, rp, col0, N);
-            }
+            for (int j = 0; j < 8; ++j) b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        tmem_wait_ld_regs(v);
+        if (c + 32 < COLS) tmem_ld_x32(t_row + c + 32, u[((c >> 5) & 1) ^ 1]);
+        float z[32];
+        scale_bias(z, v, sx, sw, b);
+        if constexpr (OUT_BF16) activate(z, epi);
+        const bool begins = !OUT_BF16 || (c & 32) == 0, ends = !OUT_BF16 || (c & 32) != 0;
+        if (begins) {
+            if (lane == 0) bulk_wait_read<1>();  // the store that last used the slab has read it
+            __syncwarp();
         }
-        uint8_t *buf = bufs + pp * kSlab;
-        if (lane == 0) bulk_wait_read<1>();  // the store that last used `buf` has read it
-        __syncwarp();
-        uint8_t *rowp = buf + lane * 128;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            uint4 w;
-            if constexpr (OUT_BF16) w = pack8(f + 8 * u);
-            else w = make_uint4(__float_as_uint(f[4 * u]), __float_as_uint(f[4 * u + 1]), __float_as_uint(f[4 * u + 2]),
-                                __float_as_uint(f[4 * u + 3]));
-            *reinterpret_cast<uint4 *>(rowp + ((u ^ (lane & 7)) << 4)) = w;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-            tma_store_2d(tm_y, buf, glu ? (n0 + c) / 2 : n0 + c, store_row);
-            bulk_commit();
-        }
-        pp ^= 1;
+        to_slab<OUT_BF16>(sl.buf + sl.pp * kSlab, z, OUT_BF16 ? (c & 32) / 8 : 0, lane);
+        if (ends) store_slab(tm_y, sl, n0 + (OUT_BF16 ? c & ~63 : c), store_row, lane);
     }
+}
+
+// Gated epilogues: 32 gate columns, then their 32 inputs; 128 accumulator columns fill a slab.
+template <int COLS>
+__device__ __forceinline__ void drain_glu(uint32_t t_row, int store_row, int n0, int N, const EpiArgs &ea, float sx,
+                                          const CUtensorMap *tm_y, Slabs &sl, int lane)
+{
+    uint32_t g[32], u[32];
+    tmem_ld_x32(t_row, g);
+    tmem_ld_x32(t_row + 32, u);
+#pragma unroll 2
+    for (int c = 0; c < COLS; c += 64) {
+        float4 sg[8], su[8], zero[8];
+        load_cols(sg, ea.sw, n0 + c, N);
+        load_cols(su, ea.sw, n0 + c + 32, N);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) zero[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        tmem_wait_ld_regs(g);
+        tmem_wait_ld_regs(u);
+        float a[32], b[32];
+        scale_bias(a, g, sx, sg, zero);
+        scale_bias(b, u, sx, su, zero);
+        if (c + 64 < COLS) {
+            tmem_ld_x32(t_row + c + 64, g);
+            tmem_ld_x32(t_row + c + 96, u);
+        }
+        activate(a, ea.epi == E_SWIGLU ? E_SWISH : E_GELU);
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) mul_f32x2(a[j], a[j + 1], b[j], b[j + 1]);
+        if ((c & 64) == 0) {
+            if (lane == 0) bulk_wait_read<1>();
+            __syncwarp();
+        }
+        to_slab<true>(sl.buf + sl.pp * kSlab, a, (c & 64) / 16, lane);
+        if ((c & 64) != 0) store_slab(tm_y, sl, (n0 + c - 64) / 2, store_row, lane);
+    }
+}
+
+// The residual's first two 32-column chunks of a tile into the two slabs, once their last
+// stores have read them: called before the wait for the accumulator.
+__device__ __forceinline__ void load_residual(const CUtensorMap *tm_r, Slabs &sl, int slab, int x, int y, int lane)
+{
+    if (lane == 0) {
+        mbar_arrive_expect_tx(&sl.bar[slab], kSlab);
+        tma_load_2d(sl.buf + slab * kSlab, tm_r, &sl.bar[slab], x, y);
+    }
+    sl.armed |= 1u << slab;
+}
+
+template <int COLS>
+__device__ __forceinline__ void start_residual(const CUtensorMap *tm_r, Slabs &sl, int n0, int store_row, int lane)
+{
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+    sl.pp = 0;
+    load_residual(tm_r, sl, 0, n0, store_row, lane);
+    load_residual(tm_r, sl, 1, n0 + 32, store_row, lane);
+    // the rest on their way to L2
+    if (lane == 0)
+        for (int c = 64; c < COLS; c += 32) tma_prefetch_l2_2d(tm_r, n0 + c, store_row);
+}
+
+// y = acc sx sw + b + residual in fp32: the residual arrives in the slab that the result leaves
+// from (read by rows it would be 16 bytes of a different line per lane).  False on a timeout.
+template <int COLS>
+__device__ __forceinline__ bool drain_residual(uint32_t t_row, int store_row, int n0, int N, const EpiArgs &ea, float sx,
+                                               const CUtensorMap *tm_y, const CUtensorMap *tm_r, Slabs &sl, int lane)
+{
+    uint32_t u[2][32];
+    tmem_ld_x32(t_row, u[0]);
+#pragma unroll 2
+    for (int c = 0; c < COLS; c += 32) {
+        uint32_t(&v)[32] = u[(c >> 5) & 1];
+        float4 sw[8], b[8];
+        load_cols(sw, ea.sw, n0 + c, N);
+        load_cols(b, ea.bias, n0 + c, N);
+        tmem_wait_ld_regs(v);
+        if (c + 32 < COLS) tmem_ld_x32(t_row + c + 32, u[((c >> 5) & 1) ^ 1]);
+        float z[32];
+        scale_bias(z, v, sx, sw, b);
+        const int slab = sl.pp;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sl.bar[slab], (sl.phase >> slab) & 1u))) {
+            tmem_wait_ld();
+            return false;
+        }
+        sl.phase ^= 1u << slab;
+        sl.armed &= ~(1u << slab);
+        const uint8_t *rowp = sl.buf + slab * kSlab + lane * 128;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float4 r = *reinterpret_cast<const float4 *>(rowp + ((k ^ (lane & 7)) << 4));
+            add_f32x2(z[4 * k], z[4 * k + 1], r.x, r.y);
+            add_f32x2(z[4 * k + 2], z[4 * k + 3], r.z, r.w);
+        }
+        to_slab<false>(sl.buf + slab * kSlab, z, 0, lane);
+        store_slab(tm_y, sl, n0 + c, store_row, lane);
+        if (c + 64 < COLS) {
+            if (lane == 0) bulk_wait_read<0>();  // this chunk's store has read the slab
+            __syncwarp();
+            load_residual(tm_r, sl, slab, n0 + c + 64, store_row, lane);
+        }
+    }
+    return true;
+}
+
+// One tile of an epilogue warp, from the wait for its accumulator on.
+template <int COLS, bool OUT_BF16>
+__device__ __forceinline__ bool finish_tile(uint64_t *acc_full, uint32_t parity, uint32_t t_row, int row, int store_row, int n0,
+                                            int M, int N, const EpiArgs &ea, const CUtensorMap *tm_y, const CUtensorMap *tm_r,
+                                            Slabs &sl, int lane)
+{
+    const float sx = row < M ? __ldg(ea.sx + row) : 0.f;  // these loads overlap the wait for the accumulator
+    const bool any = store_row < M && n0 < N;             // else nothing to store
+    if constexpr (!OUT_BF16)
+        if (ea.epi == E_RESID && any) start_residual<COLS>(tm_r, sl, n0, store_row, lane);
+    if (!__all_sync(0xffffffffu, mbar_wait(acc_full, parity))) return false;
+    tc_fence_after();
+    if (!any) return true;
+    if constexpr (OUT_BF16) {
+        if constexpr (COLS >= 128)
+            if (ea.epi >= E_SWIGLU) {
+                drain_glu<COLS>(t_row, store_row, n0, N, ea, sx, tm_y, sl, lane);
+                return true;
+            }
+    } else {
+        if (ea.epi == E_RESID) return drain_residual<COLS>(t_row, store_row, n0, N, ea, sx, tm_y, tm_r, sl, lane);
+    }
+    drain<COLS, OUT_BF16>(t_row, store_row, n0, N, ea, sx, tm_y, sl, lane);
+    return true;
+}
+
+// Before a warp leaves: residual loads still in flight land, stores complete.
+__device__ __forceinline__ void leave(Slabs &sl, int *status, int lane)
+{
+    for (int i = 0; i < 2; ++i)
+        if ((sl.armed >> i) & 1u)
+            if (!mbar_wait_drain(&sl.bar[i], (sl.phase >> i) & 1u)) report(status, DEV_TIMEOUT);
+    if (lane == 0) bulk_wait_all<0>();
+    __syncwarp();
 }
 
 // ------------------------------------------------------------------ one CTA
@@ -203,7 +333,7 @@ struct CtaCfg {
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
     static constexpr uint32_t RING = STAGES * STAGE;
     static constexpr uint32_t EPI = EPI_WARPS * 2 * kSlab;
-    static constexpr uint32_t SMEM = 1024 + RING + EPI + 256;
+    static constexpr uint32_t SMEM = 1024 + RING + EPI + 384;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -211,7 +341,8 @@ struct CtaCfg {
 template <int BN, bool OUT_BF16>
 __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
     linear_e4m3_cta(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                    const __grid_constant__ CUtensorMap tm_y, int M, int N, int K, const EpiArgs ea, int *status)
+                    const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_r, int M, int N, int K,
+                    const EpiArgs ea, int *status)
 {
     using C = CtaCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -222,7 +353,8 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
     uint64_t *empty = full + C::STAGES;
     uint64_t *acc_full = empty + C::STAGES;  // [2]
     uint64_t *acc_empty = acc_full + 2;      // [2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    uint64_t *res_bar = acc_empty + 2;       // [EPI_WARPS][2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_bar + 2 * C::EPI_WARPS);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
@@ -240,6 +372,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], C::EPI_WARPS);
         }
+        for (int b = 0; b < 2 * C::EPI_WARPS; ++b) mbar_init(&res_bar[b], 1);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_x);
@@ -329,31 +462,26 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
         }
     } else {
         const int q = warp & 3;  // TMEM lane quarter this warp may access
-        uint8_t *bufs = epi_buf + q * 2 * kSlab;
-        int acc = 0, pp = 0;
+        Slabs sl{epi_buf + q * 2 * kSlab, res_bar + 2 * q, 0, 0, 0};
+        int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
             if (*abort_flag) break;
-            const int m0 = tile / n_tiles * 128, n0 = tile % n_tiles * BN;
-            const int row = m0 + q * 32 + lane;
-            const float sx = row < M ? __ldg(ea.sx + row) : 0.f;  // overlaps the wait for the accumulator
-            if (!mbar_wait(&acc_full[acc], acc_phase)) {
+            const int m0 = tile / n_tiles * 128 + q * 32, n0 = tile % n_tiles * BN;
+            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+            if (!finish_tile<BN, OUT_BF16>(&acc_full[acc], acc_phase, t_row, m0 + lane, m0, n0, M, N, ea, &tm_y, &tm_r, sl,
+                                           lane)) {
                 report(status, DEV_TIMEOUT);
                 *abort_flag = 1;
                 break;
             }
-            tc_fence_after();
-            if (m0 + q * 32 < M)  // a warp whose rows all lie past M has nothing to store
-                drain<BN, OUT_BF16>(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, row, m0 + q * 32, n0, M, N,
-                                    ea, sx, &tm_y, bufs, pp, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[acc]);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
         }
-        if (lane == 0) bulk_wait_all<0>();
-        __syncwarp();
+        leave(sl, status, lane);
     }
 
     tc_fence_before();
@@ -378,7 +506,7 @@ struct PairCfg {
     static constexpr uint32_t STAGE = 2 * HALF;    // this CTA's x rows + w rows
     static constexpr uint32_t RING = STAGES * STAGE;
     static constexpr uint32_t EPI = EPI_WARPS * 2 * kSlab;
-    static constexpr uint32_t SMEM = 1024 + RING + EPI + 256;
+    static constexpr uint32_t SMEM = 1024 + RING + EPI + 384;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -386,7 +514,8 @@ struct PairCfg {
 template <bool OUT_BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     linear_e4m3_pair(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_y, int M, int N, int K, const EpiArgs ea, int *status)
+                     const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_r, int M, int N, int K,
+                     const EpiArgs ea, int *status)
 {
     using C = PairCfg;
     extern __shared__ uint8_t smem_raw[];
@@ -397,7 +526,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     uint64_t *empty = full + C::STAGES;                               // both CTAs
     uint64_t *acc_full = empty + C::STAGES;                           // both CTAs [2]
     uint64_t *acc_empty = acc_full + 2;                               // used in the leader [2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    uint64_t *res_bar = acc_empty + 2;       // [EPI_WARPS][2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_bar + 2 * C::EPI_WARPS);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
@@ -418,6 +548,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], 2 * C::EPI_WARPS);  // one arrival per epilogue warp of either CTA
         }
+        for (int b = 0; b < 2 * C::EPI_WARPS; ++b) mbar_init(&res_bar[b], 1);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_x);
@@ -515,33 +646,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     } else {
         const int q = warp & 3;            // TMEM lane quarter
         const int h = (warp - 2) >> 2;     // column half
-        uint8_t *bufs = epi_buf + (warp - 2) * 2 * kSlab;
+        Slabs sl{epi_buf + (warp - 2) * 2 * kSlab, res_bar + 2 * (warp - 2), 0, 0, 0};
         const uint32_t leader_acc_empty[2] = {map_to_rank(&acc_empty[0], 0), map_to_rank(&acc_empty[1], 0)};
-        int acc = 0, pp = 0;
+        int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = pair; tile < num_tiles; tile += npairs) {
             if (*abort_flag) break;
-            const int m0 = tile / n_tiles * 256 + static_cast<int>(rank) * 128;
+            const int m0 = tile / n_tiles * 256 + static_cast<int>(rank) * 128 + q * 32;
             const int n0 = tile % n_tiles * C::BN + h * C::COLS;
-            const int row = m0 + q * 32 + lane;
-            const float sx = row < M ? __ldg(ea.sx + row) : 0.f;
-            if (!mbar_wait(&acc_full[acc], acc_phase)) {
+            const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::BN + h * C::COLS;
+            if (!finish_tile<C::COLS, OUT_BF16>(&acc_full[acc], acc_phase, t_row, m0 + lane, m0, n0, M, N, ea, &tm_y, &tm_r, sl,
+                                                lane)) {
                 report(status, DEV_TIMEOUT);
                 *abort_flag = 1;
                 break;
             }
-            tc_fence_after();
-            if (m0 + q * 32 < M && n0 < N)
-                drain<C::COLS, OUT_BF16>(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::BN + h * C::COLS, row,
-                                         m0 + q * 32, n0, M, N, ea, sx, &tm_y, bufs, pp, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(leader_acc_empty[acc]);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
         }
-        if (lane == 0) bulk_wait_all<0>();
-        __syncwarp();
+        leave(sl, status, lane);
     }
 
     tc_fence_before();
@@ -567,7 +693,7 @@ cudaError_t allow_smem(Kern kern, uint32_t bytes, uint64_t (&configured)[64])
 }
 
 struct Maps {
-    CUtensorMap x, w, y;
+    CUtensorMap x, w, y, r;
 };
 
 template <int BN, bool OUT_BF16>
@@ -579,7 +705,7 @@ cudaError_t launch_cta(const Maps &t, int M, int N, int K, const EpiArgs &ea, cu
     if (e != cudaSuccess) return e;
     const int tiles = (M + 127) / 128 * ((N + BN - 1) / BN);
     return launch_k(linear_e4m3_cta<BN, OUT_BF16>, dim3(std::min(current_sm_count(), tiles)), dim3(C::THREADS), C::SMEM, s,
-                    t.x, t.w, t.y, M, N, K, ea, current_device_status_word());
+                    t.x, t.w, t.y, t.r, M, N, K, ea, current_device_status_word());
 }
 
 template <bool OUT_BF16>
@@ -591,7 +717,7 @@ cudaError_t launch_pair(const Maps &t, int M, int N, int K, const EpiArgs &ea, c
     if (e != cudaSuccess) return e;
     const int tiles = (M + 255) / 256 * ((N + C::BN - 1) / C::BN);
     const int pairs = std::max(1, std::min(current_sm_count() / 2, tiles));
-    return launch_k(linear_e4m3_pair<OUT_BF16>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, s, t.x, t.w, t.y, M, N, K, ea,
+    return launch_k(linear_e4m3_pair<OUT_BF16>, dim3(2 * pairs), dim3(C::THREADS), C::SMEM, s, t.x, t.w, t.y, t.r, M, N, K, ea,
                     current_device_status_word());
 }
 
@@ -616,11 +742,13 @@ cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, co
     if (r == FE_OK)
         r = bf16 ? make_tmap_2d(&t.y, y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, m, ny, ny, 32, 64)
                  : make_tmap_2d(&t.y, y, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, m, n, n, 32, 32);
+    t.r = t.y;  // not read without a residual
+    if (r == FE_OK && residual) r = make_tmap_2d(&t.r, residual, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, m, n, n, 32, 32);
     if (r != FE_OK) {
         *st = r;
         return cudaSuccess;
     }
-    const EpiArgs ea{sx, sw, bias, residual, epilogue};
+    const EpiArgs ea{sx, sw, bias, epilogue};
     const int M = static_cast<int>(m), N = static_cast<int>(n), K = static_cast<int>(k);
     if (pair) return bf16 ? launch_pair<true>(t, M, N, K, ea, s) : launch_pair<false>(t, M, N, K, ea, s);
     if (bn == 256) return bf16 ? launch_cta<256, true>(t, M, N, K, ea, s) : launch_cta<256, false>(t, M, N, K, ea, s);
