@@ -24,7 +24,9 @@
 //     of m-tile i is hd 16 g + 2 i).  P^T in B-fragment form is the 8x8 transpose of S^T's
 //     accumulator.
 // Each e4m3 pair becomes f16x2 in one conversion (exact).  The sequence is split over CTAs when
-// there are too few to fill the GPU; attn_cache_join sums the parts.
+// there are too few to fill the GPU.  Up to eight parts are the CTAs of a cluster, which sum them
+// through distributed shared memory; more (one long sequence) go through the workspace and
+// attn_cache_join, a launch later.
 //
 // Pages beyond the sequence are never read; slots past its end are masked before they are used
 // (values zeroed: a slot never written may hold any code).  A page id outside the pool sets
@@ -78,10 +80,28 @@ template <int HD, int NR, int WARPS>
 struct StreamCfg {
     static constexpr int ROWS = 8 * NR;
     static constexpr int LD = HD + 4;  // floats per row of the joining buffer
-    static constexpr uint32_t SMEM = WARPS * ROWS * (LD + 2) * 4;
+    static constexpr uint32_t SMEM = (WARPS * ROWS * (LD + 2) + ROWS * 2) * 4;
 };
 
-template <int HD, int NR, int WARPS>
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// CLUSTER: the launch's parts (gridDim.z of them) are one cluster along z.
+template <int HD, int NR, int WARPS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs a, int row_tiles, int *status)
 {
     using C = StreamCfg<HD, NR, WARPS>;
@@ -90,7 +110,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     constexpr int VC = HD >= 128 ? HD / 128 : 1;
     constexpr int VW = VB / 4;             // words of those
     constexpr int MT = HD / 16;            // m-tiles of O^T
-    extern __shared__ float join[];        // [WARPS][ROWS][LD], then [WARPS][ROWS][2]
+    extern __shared__ __align__(16) float join[];  // [WARPS][ROWS][LD], then [WARPS][ROWS][2], then [ROWS][2]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, c = lane & 3;
@@ -176,62 +196,82 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
         l[n][0] = l[n][1] = 0.f;
     }
 
+    // 32 tokens = two 16-token tiles, each inside one page (pages are 16 tokens or more).  K of a
+    // warp's next run is loaded when S has consumed this run's, V when O has: a load has the
+    // softmax and the other product to arrive in, at no more registers than one run's.
     const int32_t *tab = a.table + static_cast<int64_t>(b) * a.width;
     const int page_mask = (1 << a.page_log2) - 1;
-    for (int run = run0 + warp; run < run1; run += WARPS) {
-        // 32 tokens = two 16-token tiles, each inside one page (pages are 16 tokens or more)
-        uint4 kf[2][2][KC];          // [tile][token g / g + 8][chunk]
-        uint32_t vf[2][4][VC][VW];   // [tile][token 2c, 2c + 1, 2c + 8, 2c + 9][chunk][word]
-        float sk[2], sv[2];
-        bool have[2];
+    uint4 kf[2][2][KC];         // [tile][token g / g + 8][chunk]
+    uint32_t vf[2][4][VC][VW];  // [tile][token 2c, 2c + 1, 2c + 8, 2c + 9][chunk][word]
+    int id[2], id_next[2];      // pages of the run in the registers and of the one after it, -1: none
+    float sk[2], sv[2], sk_next[2], sv_next[2];
+    auto look_up = [&](int run, int (&page)[2]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int tok = run * kWarpTokens + 16 * u;
-            int id = -1;
-            if (tok < end_all) {
-                id = __ldg(tab + (tok >> a.page_log2));
-                if (id < 0 || id >= a.pages) {
+            page[u] = -1;
+            if (run < run1 && tok < end_all) {
+                page[u] = __ldg(tab + (tok >> a.page_log2));
+                if (page[u] < 0 || page[u] >= a.pages) {
                     if (lane == 0) report(status, DEV_BAD_INPUT);
-                    id = -1;
+                    page[u] = -1;
                 }
-            }
-            have[u] = id >= 0;
-            if (have[u]) {
-                const int64_t ph = static_cast<int64_t>(id) * a.kv_heads + kvh;
-                const int64_t at = ((ph << a.page_log2) + (tok & page_mask)) * HD;
-                const uint8_t *kp = a.k + at + g * HD + 16 * c, *vp = a.v + at + 2 * c * HD + VB * g;
-#pragma unroll
-                for (int j = 0; j < KC; ++j) {
-                    kf[u][0][j] = ld_stream16(kp + 64 * j);
-                    kf[u][1][j] = ld_stream16(kp + 8 * HD + 64 * j);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < VC; ++j) {
-                        const uint8_t *p = vp + ((i & 1) + 8 * (i >> 1)) * HD + 128 * j;
-                        if constexpr (VB == 16) {
-                            const uint4 x = ld_stream16(p);
-                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y, vf[u][i][j][2] = x.z, vf[u][i][j][3] = x.w;
-                        } else {
-                            const uint2 x = ld_stream8(p);
-                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y;
-                        }
-                    }
-                sk[u] = __ldg(a.ks + ph);
-                sv[u] = __ldg(a.vs + ph);
-            } else {
-                sk[u] = sv[u] = 0.f;
-#pragma unroll
-                for (int j = 0; j < KC; ++j) kf[u][0][j] = kf[u][1][j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < VC; ++j)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vf[u][i][j][w] = 0;
             }
         }
+    };
+    auto codes_at = [&](int run, int u, int page) -> int64_t {
+        const int64_t ph = static_cast<int64_t>(page) * a.kv_heads + kvh;
+        return ((ph << a.page_log2) + ((run * kWarpTokens + 16 * u) & page_mask)) * HD;
+    };
+    auto load_k = [&](int run, const int (&page)[2], float (&ks)[2], float (&vs)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (page[u] >= 0) {
+                const uint8_t *p = a.k + codes_at(run, u, page[u]) + g * HD + 16 * c;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+                    kf[u][0][j] = ld_stream16(p + 64 * j);
+                    kf[u][1][j] = ld_stream16(p + 8 * HD + 64 * j);
+                }
+                const int64_t ph = static_cast<int64_t>(page[u]) * a.kv_heads + kvh;
+                ks[u] = __ldg(a.ks + ph);
+                vs[u] = __ldg(a.vs + ph);
+            } else {
+                ks[u] = vs[u] = 0.f;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) kf[u][0][j] = kf[u][1][j] = make_uint4(0, 0, 0, 0);
+            }
+        }
+    };
+    auto load_v = [&](int run, const int (&page)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint8_t *p = page[u] >= 0 ? a.v + codes_at(run, u, page[u]) + 2 * c * HD + VB * g : nullptr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < VC; ++j) {
+                    if (page[u] >= 0) {
+                        const uint8_t *q = p + ((i & 1) + 8 * (i >> 1)) * HD + 128 * j;
+                        if constexpr (VB == 16) {
+                            const uint4 x = ld_stream16(q);
+                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y, vf[u][i][j][2] = x.z, vf[u][i][j][3] = x.w;
+                        } else {
+                            const uint2 x = ld_stream8(q);
+                            vf[u][i][j][0] = x.x, vf[u][i][j][1] = x.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vf[u][i][j][w] = 0;
+                    }
+                }
+        }
+    };
+    look_up(run0 + warp, id);
+    load_k(run0 + warp, id, sk, sv);
+    load_v(run0 + warp, id);
+    look_up(run0 + warp + WARPS, id_next);
+    for (int run = run0 + warp; run < run1; run += WARPS) {
         // S^T: accumulator (token g, row 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1)
         float s[NR][2][4];
 #pragma unroll
@@ -254,6 +294,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                     for (int n = 0; n < NR; ++n) mma_f16(s[n][u], a0, a1, a2, a3, qf[n][j][q][0], qf[n][j][q][1]);
                 }
             }
+        load_k(run + WARPS, id_next, sk_next, sv_next);
         // base-2 logits, masked; t = s + log2 sv (a page of zero values adds nothing: log2 -> 0)
         float ev[2];
 #pragma unroll
@@ -267,7 +308,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int tok = run * kWarpTokens + 16 * u + g + 8 * (i >> 1);
-                    const bool on = have[u] && tok <= lim[n][i & 1];
+                    const bool on = id[u] >= 0 && tok <= lim[n][i & 1];
                     s[n][u][i] = on ? s[n][u][i] * (sk[u] * qs[n][i & 1]) : -INFINITY;
                     top[i & 1] = fmaxf(top[i & 1], s[n][u][i] + ev[u]);
                 }
@@ -341,10 +382,14 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                         mma_f16(o[n][2 * VW * j + 2 * w + 1], b0, b1, b2, b3, pt[n][u][0], pt[n][u][1]);
                     }
                 }
+        load_v(run + WARPS, id_next);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) id[u] = id_next[u], sk[u] = sk_next[u], sv[u] = sv_next[u];
+        look_up(run + 2 * WARPS, id_next);
     }
 
     // join the warps: each leaves its rows' m, l and O, then the CTA sums them
-    float *ml = join + WARPS * C::ROWS * C::LD;
+    float *ml = join + WARPS * C::ROWS * C::LD, *cml = ml + WARPS * C::ROWS * 2;
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -387,6 +432,11 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                 acc.x += x.x * k, acc.y += x.y * k, acc.z += x.z * k, acc.w += x.w * k;
             }
         }
+        if constexpr (CLUSTER) {  // this CTA's part, for the cluster to read
+            *reinterpret_cast<float4 *>(join + r * C::LD + hd) = acc;  // only this thread has read it
+            if (hd == 0) *reinterpret_cast<float2 *>(cml + 2 * r) = make_float2(m, sum);
+            continue;
+        }
         const int64_t orow = (sq.t0 + (r0 + r) / a.group) * static_cast<int64_t>(a.q_heads) + kvh * a.group + (r0 + r) % a.group;
         if (a.splits == 1) {
             const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a row that sees nothing is zero
@@ -397,6 +447,34 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
             *reinterpret_cast<float4 *>(a.part_o + at * HD + hd) = acc;
             if (hd == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, sum);
         }
+    }
+    if constexpr (CLUSTER) {
+        const int parts = gridDim.z;
+        __syncthreads();
+        cluster_sync();  // every part is in its CTA's shared memory
+        for (int i = split + parts * threadIdx.x; i < C::ROWS * HD / 4; i += parts * 32 * WARPS) {
+            const int r = i / (HD / 4), hd = i % (HD / 4) * 4;
+            if (r0 + r >= rows) break;
+            float m = -INFINITY;
+            for (int k = 0; k < parts; ++k) m = fmaxf(m, ld_cluster2(map_to_rank(cml + 2 * r, k)).x);
+            float sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < parts; ++k) {
+                const float2 p = ld_cluster2(map_to_rank(cml + 2 * r, k));
+                if (p.x == -INFINITY && p.y == 0.f) continue;  // saw nothing
+                const float f = p.x == -INFINITY ? 1.f : exp2_fast(p.x - m);
+                const float4 x = ld_cluster4(map_to_rank(join + r * C::LD + hd, k));
+                sum += p.y * f;
+                acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+            }
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            const int64_t orow =
+                (sq.t0 + (r0 + r) / a.group) * static_cast<int64_t>(a.q_heads) + kvh * a.group + (r0 + r) % a.group;
+            *reinterpret_cast<uint2 *>(a.out + orow * HD + hd) =
+                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        }
+        __syncthreads();
+        cluster_sync();  // no CTA leaves while another reads its part
     }
 }
 
@@ -445,65 +523,112 @@ cudaError_t launch_join(const CacheArgs &a, int head_dim, int *status, cudaStrea
     return head_dim == 64 ? launch_join<64>(a, status, s) : head_dim == 128 ? launch_join<128>(a, status, s) : launch_join<256>(a, status, s);
 }
 
-constexpr int kWarps = 4;
-constexpr int kStreamRows = 32;  // rows of a key-value head up to which the streaming kernel runs
+constexpr int kStreamRows = 32;    // rows of a key-value head up to which the streaming kernel runs
+constexpr int kClusterParts = 8;   // portable cluster size
+constexpr int kPartTokens = 128;   // a part has a run for each of four warps
 
 // 8-row tiles of a CTA: 16 rows where the registers allow it and there are more than 8
-int row_tile_count(int rows, int head_dim) { return rows > 8 && head_dim < 256 ? 2 : 1; }
-
-template <int HD, int NR>
-cudaError_t stream(const CacheArgs &a, int *status, cudaStream_t s)
-{
-    using C = StreamCfg<HD, NR, kWarps>;
-    static_assert(C::SMEM <= 48 * 1024, "no opt-in shared memory");
-    const int row_tiles = (a.max_len * a.group + C::ROWS - 1) / C::ROWS;
-    cudaError_t e = launch_k(attn_cache_stream<HD, NR, kWarps>,
-                             dim3(static_cast<unsigned>(a.batch) * row_tiles, a.kv_heads, a.splits), dim3(32 * kWarps),
-                             C::SMEM, s, a, row_tiles, status);
-    return e != cudaSuccess || a.splits == 1 ? e : launch_join<HD>(a, status, s);
-}
-
-template <int HD>
-cudaError_t stream_any(const CacheArgs &a, int *status, cudaStream_t s)
-{
-    if constexpr (HD < 256)
-        if (row_tile_count(a.max_len * a.group, HD) == 2) return stream<HD, 2>(a, status, s);
-    return stream<HD, 1>(a, status, s);
-}
-
-}  // namespace
+int row_tile_count(int64_t rows, int head_dim) { return rows > 8 && head_dim < 256 ? 2 : 1; }
 
 // Which kernel runs and into how many parts the sequences are split.  A matter of the arguments
 // alone (a B200 has kSms multiprocessors), so that a workspace sized on one device serves on any.
 struct CachePlan {
-    bool tiles;
+    bool tiles, cluster, wide;  // cluster: the parts are a cluster; wide: eight warps a CTA
     int splits;
+    bool workspace() const { return splits > 1 && !cluster; }
 };
 CachePlan plan_attention_cache(int batch, int max_len, int max_kv, int q_heads, int kv_heads, int head_dim)
 {
     const int64_t rows = static_cast<int64_t>(max_len) * (q_heads / kv_heads);
-    CachePlan p;
-    p.tiles = rows > kStreamRows;
-    int64_t want;
+    CachePlan p{rows > kStreamRows, false, false, 1};
     if (p.tiles) {
         const int64_t tiles = (rows + attention_cache_tile_rows(head_dim) - 1) / attention_cache_tile_rows(head_dim);
         // one CTA an SM: split until they have one each, 512 tokens or more a part
-        want = std::min<int64_t>(kSms / std::max<int64_t>(1, tiles * batch * kv_heads), 65535 / tiles);
-    } else {
-        // enough CTAs for about four rounds of the resident ones (sequences differ in length)
-        const int per = 8 * row_tile_count(static_cast<int>(rows), head_dim);
-        const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
-        want = (12ll * kSms + ctas - 1) / ctas;
+        const int64_t want = std::min<int64_t>(kSms / std::max<int64_t>(1, tiles * batch * kv_heads), 65535 / tiles);
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+        return p;
     }
-    p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+    const int per = 8 * row_tile_count(rows, head_dim);
+    const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
+    constexpr int64_t resident = 3 * kSms;
+    if (ctas < resident && max_kv <= 2048 * std::min<int64_t>(resident / ctas, kClusterParts)) {
+        // As many parts as all fit at once, and those short.  (Beside more CTAs than that clusters wait for room: 7 parts of
+        // 32 sequences x 8 heads took 186 us as clusters and 158 with the second launch, one sequence of
+        // 2,000 tokens 8.5 and 14.9.)
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({resident / ctas, kClusterParts, max_kv / kPartTokens})));
+        p.cluster = p.splits > 1;
+    }
+    if (p.splits == 1) {
+        // About four rounds of the resident CTAs: sequences differ in length.  Measured on 32 sequences of
+        // 8,000 to 16,000 tokens, 8 heads: 1 round 200 us, 2 168, 4 158, 8 165, 16 190 (a CTA costs 2.7 us
+        // beside its reading).
+        const int64_t want = (4 * resident + ctas - 1) / ctas;
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+    }
+    // a CTA that has its SM to itself takes twice the warps
+    p.wide = head_dim < 256 && ctas * p.splits <= kSms;
     return p;
 }
+
+template <int HD, int NR, int WARPS, bool CLUSTER>
+cudaError_t stream(const CacheArgs &a, int *status, cudaStream_t s)
+{
+    using C = StreamCfg<HD, NR, WARPS>;
+    auto kern = attn_cache_stream<HD, NR, WARPS, CLUSTER>;
+    if constexpr (C::SMEM > 48 * 1024) {
+        static uint64_t configured[64] = {};  // context the attribute was set in
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const uint64_t ctx = current_context_id();
+        if (dev >= 64 || configured[dev] != ctx) {
+            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            if (e != cudaSuccess) return e;
+            if (dev < 64) configured[dev] = ctx;
+        }
+    }
+    const int row_tiles = (a.max_len * a.group + C::ROWS - 1) / C::ROWS;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = a.splits;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * row_tiles, a.kv_heads, a.splits);
+    cfg.blockDim = dim3(32 * WARPS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = CLUSTER ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, row_tiles, status);
+    return e != cudaSuccess || CLUSTER || a.splits == 1 ? e : launch_join<HD>(a, status, s);
+}
+
+template <int HD, int NR>
+cudaError_t stream_as(const CacheArgs &a, const CachePlan &p, int *status, cudaStream_t s)
+{
+    if constexpr (HD < 256) {
+        if (p.wide) return p.cluster ? stream<HD, NR, 8, true>(a, status, s) : stream<HD, NR, 8, false>(a, status, s);
+    }
+    return p.cluster ? stream<HD, NR, 4, true>(a, status, s) : stream<HD, NR, 4, false>(a, status, s);
+}
+
+template <int HD>
+cudaError_t stream_any(const CacheArgs &a, const CachePlan &p, int *status, cudaStream_t s)
+{
+    if constexpr (HD < 256)
+        if (row_tile_count(static_cast<int64_t>(a.max_len) * a.group, HD) == 2) return stream_as<HD, 2>(a, p, status, s);
+    return stream_as<HD, 1>(a, p, status, s);
+}
+
+}  // namespace
 
 size_t attention_cache_workspace_bytes(int batch, int max_len, int64_t total, int max_kv, int q_heads, int kv_heads,
                                        int head_dim)
 {
-    const int64_t splits = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim).splits;
-    return splits == 1 ? 0 : static_cast<size_t>(total) * q_heads * splits * (head_dim + 2) * sizeof(float);
+    const CachePlan p = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
+    return p.workspace() ? static_cast<size_t>(total) * q_heads * p.splits * (head_dim + 2) * sizeof(float) : 0;
 }
 
 cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int batch, int max_len, int64_t total,
@@ -534,9 +659,9 @@ cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int 
         cudaError_t e = launch_attention_cache_tiles(a, head_dim, status, s, st);
         return e != cudaSuccess || *st != FE_OK || a.splits == 1 ? e : launch_join(a, head_dim, status, s);
     }
-    if (head_dim == 64) return stream_any<64>(a, status, s);
-    if (head_dim == 128) return stream_any<128>(a, status, s);
-    return stream_any<256>(a, status, s);
+    if (head_dim == 64) return stream_any<64>(a, plan, status, s);
+    if (head_dim == 128) return stream_any<128>(a, plan, status, s);
+    return stream_any<256>(a, plan, status, s);
 }
 
 }  // namespace fe

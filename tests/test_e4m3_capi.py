@@ -86,16 +86,17 @@ def test_attention_cache_workspace(fe_lib):
     ask = lambda batch, max_len, total, kv, hq, hkv, hd: (
         fe_lib.fe_attention_cache_workspace_bytes(batch, max_len, total, kv, hq, hkv, hd, C.byref(size)), size.value)
     assert ask(1, 1, 1, 100, 16, 8, 128) == (0, 0)          # too short to split
-    status, need = ask(1, 1, 1, 16000, 16, 8, 128)          # one token over a long cache is
-    assert status == 0 and need >= 16 * 2 * 130 * 4
+    assert ask(1, 1, 1, 16000, 16, 8, 128) == (0, 0)        # eight parts or fewer meet in a cluster
+    status, need = ask(1, 1, 1, 64000, 16, 8, 128)          # one token over a very long cache
+    assert status == 0 and need >= 16 * 9 * 130 * 4
     assert ask(8, 2000, 16000, 3000, 16, 8, 128) == (0, 0)  # enough CTAs without
     assert ask(0, 0, 0, 0, 16, 8, 128) == (0, 0)
     assert ask(1, 1, 1, -1, 16, 8, 128)[0] == 1 and ask(1, 1, 1, 10, 16, 8, 80)[0] == 4
     assert fe_lib.fe_attention_cache_workspace_bytes(1, 1, 1, 1, 1, 1, 64, None) == 1
-    assert _attend(fe_lib, max_kv=16000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8) == 1
+    assert _attend(fe_lib, max_kv=64000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8) == 1
     assert b"workspace" in fe_lib.fe_last_error_message()
-    assert _attend(fe_lib, max_kv=16000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8, ws=buf, ws_bytes=need - 1) == 1
-    assert _attend(fe_lib, max_kv=16000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8, ws=odd, ws_bytes=need) == 1
+    assert _attend(fe_lib, max_kv=64000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8, ws=buf, ws_bytes=need - 1) == 1
+    assert _attend(fe_lib, max_kv=64000, batch=1, total=1, max_len=1, hd=128, hq=16, hkv=8, ws=odd, ws_bytes=need) == 1
     assert _attend(fe_lib, scale=float("inf")) == 1 and _attend(fe_lib, max_kv=-1) == 1 and _attend(fe_lib, out=None) == 1
 
 

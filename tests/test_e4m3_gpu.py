@@ -277,7 +277,7 @@ def _attend(b, ops, cache, causal=True, scale=None, check=None):
     return out
 
 
-ATTENDS = [([1], [0]), ([1], [1]), ([1], [700]), ([1, 1, 1], [5, 64, 2500]), ([0, 7, 0, 1], [3, 60, 0, 15]), ([3, 1], [13, 0]),
+ATTENDS = [([1], [0]), ([1], [1]), ([1], [700]), ([1], [9000]), ([2], [40000]), ([1, 1, 1], [5, 64, 2500]), ([0, 7, 0, 1], [3, 60, 0, 15]), ([3, 1], [13, 0]),
            ([130, 1, 64], [0, 500, 77]), ([17, 33, 65, 128], [15, 31, 63, 127]), ([300], [0]), ([257, 129], [1000, 3])]
 
 
