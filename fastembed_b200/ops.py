@@ -4,6 +4,7 @@ FeError on a non-OK status.  PyTorch only supplies device memory and streams."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import numpy as np
@@ -326,12 +327,15 @@ def _matrix(t, name, dtype=None):
 
 def _launch(dev, name, *args):
     """One C ABI call on CUDA device `dev` and that device's current torch stream."""
+    fn = getattr(capi._lib or capi.lib(), name)
     stream = torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without its Stream object
-    if torch.cuda.current_device() == dev:
-        call(name, *args, stream)
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            call(name, *args, stream)
+            status = fn(*args, stream)
+    if status != capi.FE_OK:
+        capi.check(status, name)
 
 
 _KIND = {torch.float32: DTYPE["f32"], torch.bfloat16: DTYPE["bf16"]}
@@ -397,21 +401,30 @@ def _cache_args(qkv, cu_seqlens, past_lens, page_table, cache, q_heads):
     dev = k.get_device()
     if k.dim() != 4:
         raise ValueError(f"cache.k: expected [pages, kv_heads, page_size, head_dim], got {tuple(k.shape)}")
-    pages, kv_heads, page, hd = k.shape
-    _check(k, "cache.k", F8, k.shape, dev)
-    _check(v, "cache.v", F8, k.shape, dev)
-    _check(ks, "cache.k_scale", torch.float32, (pages, kv_heads), dev)
-    _check(vs, "cache.v_scale", torch.float32, (pages, kv_heads), dev)
+    shape = k.shape
+    pages, kv_heads, page, hd = shape
     T = qkv.shape[0]
-    _check(qkv, "qkv", torch.bfloat16, (T, (q_heads + 2 * kv_heads) * hd), dev)
     batch = cu_seqlens.shape[0] - 1
     if batch < 0:
         raise ValueError("cu_seqlens: expected batch + 1 offsets")
     width = page_table.shape[-1]
+    _check(k, "cache.k", F8, shape, dev)
+    _check(v, "cache.v", F8, shape, dev)
+    _check(ks, "cache.k_scale", torch.float32, shape[:2], dev)
+    _check(vs, "cache.v_scale", torch.float32, shape[:2], dev)
+    _check(qkv, "qkv", torch.bfloat16, (T, (q_heads + 2 * kv_heads) * hd), dev)
     _check(cu_seqlens, "cu_seqlens", torch.int32, (batch + 1,), dev)
     _check(past_lens, "past_lens", torch.int32, (batch,), dev)
     _check(page_table, "page_table", torch.int32, (batch, width), dev)
     return dev, T, batch, kv_heads, hd, width, pages, page
+
+
+@functools.lru_cache(maxsize=4096)
+def _cache_workspace(batch, max_len, T, max_kv_len, q_heads, kv_heads, hd):
+    """Workspace bytes of an attention call: a matter of these sizes alone."""
+    size = C.c_size_t(0)
+    call("fe_attention_cache_workspace_bytes", batch, max_len, T, max_kv_len, q_heads, kv_heads, hd, C.byref(size))
+    return size.value
 
 
 def kv_cache_append_e4m3(qkv, cu_seqlens, max_len, past_lens, page_table, cache, q_heads):
@@ -437,9 +450,7 @@ def attention_cache_e4m3(qkv, cu_seqlens, max_len, past_lens, max_kv_len, page_t
         out = torch.empty((T, q_heads * hd), dtype=torch.bfloat16, device=qkv.device)
     else:
         _check(out, "out", torch.bfloat16, (T, q_heads * hd), dev)
-    size = C.c_size_t(0)
-    call("fe_attention_cache_workspace_bytes", batch, max_len, T, max_kv_len, q_heads, kv_heads, hd, C.byref(size))
-    size = size.value
+    size = _cache_workspace(batch, max_len, T, max_kv_len, q_heads, kv_heads, hd)
     ws = torch.empty(size, dtype=torch.uint8, device=qkv.device) if size else None
     _launch(dev, "fe_attention_cache_e4m3", qkv.data_ptr(), cu_seqlens.data_ptr(), batch, max_len, T, q_heads, kv_heads, hd,
             past_lens.data_ptr(), max_kv_len, page_table.data_ptr(), width, k.data_ptr(), v.data_ptr(), ks.data_ptr(),
