@@ -70,26 +70,40 @@ struct EpiArgs {
     int epi;
 };
 
-// 32 values of a column vector from col0 on, 0 past N (a multiple of 8)
-__device__ __forceinline__ void load_cols(float4 (&v)[8], const float *__restrict__ p, int col0, int N)
+// A warp's columns' scales and biases, for the tile at hand, in its own shared memory: every lane
+// needs every column's (lane = row).  Taken before the wait for the accumulator.
+template <int COLS>
+__device__ __forceinline__ void stage_cols(float *cols, const float *__restrict__ sw, const float *__restrict__ bias, int n0,
+                                           int N, int lane)
 {
+    __syncwarp();  // the previous tile's have been read
+    float s[COLS / 32], b[COLS / 32];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        v[j] = col0 + 4 * j < N ? __ldg(reinterpret_cast<const float4 *>(p + col0 + 4 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < COLS / 32; ++i) {
+        const int col = n0 + 32 * i + lane;
+        s[i] = col < N ? __ldg(sw + col) : 0.f;
+        b[i] = col < N && bias != nullptr ? __ldg(bias + col) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < COLS / 32; ++i) {
+        cols[32 * i + lane] = s[i];
+        cols[COLS + 32 * i + lane] = b[i];
+    }
+    __syncwarp();
 }
 
-// z_j = acc_j * (sx_i sw_j) + b_j for 32 accumulator columns
-__device__ __forceinline__ void scale_bias(float (&z)[32], const uint32_t (&u)[32], float sx, const float4 (&sw)[8],
-                                           const float4 (&b)[8])
+// z_j = acc_j * (sx_i sw_j) + b_j for 32 accumulator columns, sw and b in shared memory
+__device__ __forceinline__ void scale_bias(float (&z)[32], const uint32_t (&u)[32], float sx, const float *sw, const float *b)
 {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float s0 = sw[j].x, s1 = sw[j].y, s2 = sw[j].z, s3 = sw[j].w;
-        mul_f32x2(s0, s1, sx, sx);
-        mul_f32x2(s2, s3, sx, sx);
-        fma_f32x2v(z[4 * j], z[4 * j + 1], __uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), s0, s1, b[j].x, b[j].y);
-        fma_f32x2v(z[4 * j + 2], z[4 * j + 3], __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]), s2, s3, b[j].z,
-                   b[j].w);
+        float4 s = *reinterpret_cast<const float4 *>(sw + 4 * j);
+        const float4 c = *reinterpret_cast<const float4 *>(b + 4 * j);
+        mul_f32x2(s.x, s.y, sx, sx);
+        mul_f32x2(s.z, s.w, sx, sx);
+        fma_f32x2v(z[4 * j], z[4 * j + 1], __uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), s.x, s.y, c.x, c.y);
+        fma_f32x2v(z[4 * j + 2], z[4 * j + 3], __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]), s.z, s.w, c.z,
+                   c.w);
     }
 }
 
@@ -127,11 +141,12 @@ __device__ __forceinline__ void to_slab(uint8_t *slab, const float (&z)[32], int
     }
 }
 
-// What an epilogue warp carries from tile to tile: its two 32-row x 128-byte slabs (128B-swizzled)
-// and, for the residual, a barrier each whose phase is the parity bit of `phase`.
+// What an epilogue warp carries from tile to tile: its two 32-row x 128-byte slabs (128B-swizzled),
+// its columns' vectors and, for the residual, a barrier each whose phase is the parity bit of `phase`.
 struct Slabs {
     uint8_t *buf;
     uint64_t *bar;
+    float *cols;  // scales, then biases, of the tile's columns
     uint32_t phase, armed;
     int pp;
 };
@@ -148,10 +163,9 @@ __device__ __forceinline__ void store_slab(const CUtensorMap *tm_y, Slabs &sl, i
 }
 
 // Drains COLS columns of one warp's 32 accumulator rows; rows >= M and columns >= N are clipped
-// by the tensor map.  The next 32 columns' TMEM load and this 32's column vectors are in flight
-// before the arithmetic that needs them: with loads issued where they were used (and three
-// operations in place of two for scale and bias), gelu at 26,508 x 4,096 x 1,024 took 124 us,
-// now GELU_US; the mainloop alone needs 67.
+// by the tensor map.  The next 32 columns' TMEM load is in flight during the arithmetic of these.
+// At K = 1024 this bounds the kernel: 26,508 x 4,096 with gelu takes 116 us, 67 us of it MMAs
+// (with the column vectors read from global memory where they were used: 124 us).
 template <int COLS, bool OUT_BF16>
 __device__ __forceinline__ void drain(uint32_t t_row, int store_row, int n0, int N, const EpiArgs &ea, float sx,
                                       const CUtensorMap *tm_y, Slabs &sl, int lane)
@@ -162,16 +176,10 @@ __device__ __forceinline__ void drain(uint32_t t_row, int store_row, int n0, int
 #pragma unroll 2
     for (int c = 0; c < COLS; c += 32) {
         uint32_t(&v)[32] = u[(c >> 5) & 1];
-        float4 sw[8], b[8];
-        load_cols(sw, ea.sw, n0 + c, N);
-        if (epi != E_NONE) load_cols(b, ea.bias, n0 + c, N);
-        else
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         tmem_wait_ld_regs(v);
         if (c + 32 < COLS) tmem_ld_x32(t_row + c + 32, u[((c >> 5) & 1) ^ 1]);
         float z[32];
-        scale_bias(z, v, sx, sw, b);
+        scale_bias(z, v, sx, sl.cols + c, sl.cols + COLS + c);
         if constexpr (OUT_BF16) activate(z, epi);
         const bool begins = !OUT_BF16 || (c & 32) == 0, ends = !OUT_BF16 || (c & 32) != 0;
         if (begins) {
@@ -193,16 +201,11 @@ __device__ __forceinline__ void drain_glu(uint32_t t_row, int store_row, int n0,
     tmem_ld_x32(t_row + 32, u);
 #pragma unroll 2
     for (int c = 0; c < COLS; c += 64) {
-        float4 sg[8], su[8], zero[8];
-        load_cols(sg, ea.sw, n0 + c, N);
-        load_cols(su, ea.sw, n0 + c + 32, N);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) zero[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         tmem_wait_ld_regs(g);
         tmem_wait_ld_regs(u);
         float a[32], b[32];
-        scale_bias(a, g, sx, sg, zero);
-        scale_bias(b, u, sx, su, zero);
+        scale_bias(a, g, sx, sl.cols + c, sl.cols + COLS + c);  // the biases are 0
+        scale_bias(b, u, sx, sl.cols + c + 32, sl.cols + COLS + c + 32);
         if (c + 64 < COLS) {
             tmem_ld_x32(t_row + c + 64, g);
             tmem_ld_x32(t_row + c + 96, u);
@@ -254,13 +257,10 @@ __device__ __forceinline__ bool drain_residual(uint32_t t_row, int store_row, in
 #pragma unroll 2
     for (int c = 0; c < COLS; c += 32) {
         uint32_t(&v)[32] = u[(c >> 5) & 1];
-        float4 sw[8], b[8];
-        load_cols(sw, ea.sw, n0 + c, N);
-        load_cols(b, ea.bias, n0 + c, N);
         tmem_wait_ld_regs(v);
         if (c + 32 < COLS) tmem_ld_x32(t_row + c + 32, u[((c >> 5) & 1) ^ 1]);
         float z[32];
-        scale_bias(z, v, sx, sw, b);
+        scale_bias(z, v, sx, sl.cols + c, sl.cols + COLS + c);
         const int slab = sl.pp;
         if (!__all_sync(0xffffffffu, mbar_wait(&sl.bar[slab], (sl.phase >> slab) & 1u))) {
             tmem_wait_ld();
@@ -294,6 +294,7 @@ __device__ __forceinline__ bool finish_tile(uint64_t *acc_full, uint32_t parity,
 {
     const float sx = row < M ? __ldg(ea.sx + row) : 0.f;  // these loads overlap the wait for the accumulator
     const bool any = store_row < M && n0 < N;             // else nothing to store
+    if (any) stage_cols<COLS>(sl.cols, ea.sw, ea.epi == E_NONE ? nullptr : ea.bias, n0, N, lane);
     if constexpr (!OUT_BF16)
         if (ea.epi == E_RESID && any) start_residual<COLS>(tm_r, sl, n0, store_row, lane);
     if (!__all_sync(0xffffffffu, mbar_wait(acc_full, parity))) return false;
@@ -327,13 +328,14 @@ template <int BN>
 struct CtaCfg {
     static constexpr int EPI_WARPS = 4;
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 7;
     static constexpr uint32_t A_BYTES = 128 * BK;
     static constexpr uint32_t B_BYTES = BN * BK;
     static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
     static constexpr uint32_t RING = STAGES * STAGE;
     static constexpr uint32_t EPI = EPI_WARPS * 2 * kSlab;
-    static constexpr uint32_t SMEM = 1024 + RING + EPI + 384;
+    static constexpr uint32_t COLV = EPI_WARPS * 2 * BN * 4;  // column vectors
+    static constexpr uint32_t SMEM = 1024 + RING + EPI + COLV + 384;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -349,7 +351,8 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem;
     uint8_t *epi_buf = smem + C::RING;
-    uint64_t *full = reinterpret_cast<uint64_t *>(epi_buf + C::EPI);
+    float *colv = reinterpret_cast<float *>(epi_buf + C::EPI);
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi_buf + C::EPI + C::COLV);
     uint64_t *empty = full + C::STAGES;
     uint64_t *acc_full = empty + C::STAGES;  // [2]
     uint64_t *acc_empty = acc_full + 2;      // [2]
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
         }
     } else {
         const int q = warp & 3;  // TMEM lane quarter this warp may access
-        Slabs sl{epi_buf + q * 2 * kSlab, res_bar + 2 * q, 0, 0, 0};
+        Slabs sl{epi_buf + q * 2 * kSlab, res_bar + 2 * q, colv + q * 2 * BN, 0, 0, 0};
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
 // own 128 rows of x and of w.  Both CTAs' loads complete on the leader's stage barrier, commits
 // are multicast to both CTAs' barriers, and each epilogue warp reports back to the leader.
 struct PairCfg {
-    static constexpr int STAGES = 5;
+    static constexpr int STAGES = 4;
     static constexpr int EPI_WARPS = 8;  // two per TMEM lane quarter, 128 columns each
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
     static constexpr int BN = 256;
@@ -506,7 +509,8 @@ struct PairCfg {
     static constexpr uint32_t STAGE = 2 * HALF;    // this CTA's x rows + w rows
     static constexpr uint32_t RING = STAGES * STAGE;
     static constexpr uint32_t EPI = EPI_WARPS * 2 * kSlab;
-    static constexpr uint32_t SMEM = 1024 + RING + EPI + 384;
+    static constexpr uint32_t COLV = EPI_WARPS * 2 * COLS * 4;  // column vectors
+    static constexpr uint32_t SMEM = 1024 + RING + EPI + COLV + 384;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -522,7 +526,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = smem;
     uint8_t *epi_buf = smem + C::RING;
-    uint64_t *full = reinterpret_cast<uint64_t *>(epi_buf + C::EPI);  // used in the leader
+    float *colv = reinterpret_cast<float *>(epi_buf + C::EPI);
+    uint64_t *full = reinterpret_cast<uint64_t *>(epi_buf + C::EPI + C::COLV);  // used in the leader
     uint64_t *empty = full + C::STAGES;                               // both CTAs
     uint64_t *acc_full = empty + C::STAGES;                           // both CTAs [2]
     uint64_t *acc_empty = acc_full + 2;                               // used in the leader [2]
@@ -646,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     } else {
         const int q = warp & 3;            // TMEM lane quarter
         const int h = (warp - 2) >> 2;     // column half
-        Slabs sl{epi_buf + (warp - 2) * 2 * kSlab, res_bar + 2 * (warp - 2), 0, 0, 0};
+        Slabs sl{epi_buf + (warp - 2) * 2 * kSlab, res_bar + 2 * (warp - 2), colv + (warp - 2) * 2 * C::COLS, 0, 0, 0};
         const uint32_t leader_acc_empty[2] = {map_to_rank(&acc_empty[0], 0), map_to_rank(&acc_empty[1], 0)};
         int acc = 0;
         uint32_t acc_phase = 0;
