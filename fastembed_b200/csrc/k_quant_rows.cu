@@ -22,6 +22,7 @@ namespace fe {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kWarpRowThreads = 128;  // of a block of warps with a row each: 26,508 x 1,024 and 71,550 x 2,048 within 2 % of 256
 
 __device__ __forceinline__ void load8(const float *p, float (&v)[8])
 {
@@ -60,7 +61,7 @@ __device__ __forceinline__ float row_reduce(float v, float *red)
 // IT: the input (quantiser) or the residual branch y (norm) element; BLOCK: a block per row,
 // else a warp; CH: 8-value chunks per thread.
 template <class IT, bool NORM, bool BLOCK, int CH>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(BLOCK ? kRowThreads : kWarpRowThreads)
     rows_to_e4m3(const IT *__restrict__ x, float *h32, const float *__restrict__ w, float wadd, float eps, int64_t rows,
                  int dim, uint8_t *__restrict__ q, float *__restrict__ scale)
 {
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(kRowThreads)
     __shared__ float red[kRowThreads / 32];
     const int t = BLOCK ? threadIdx.x : threadIdx.x & 31;
     const int64_t r = BLOCK ? static_cast<int64_t>(blockIdx.x)
-                            : static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
+                            : static_cast<int64_t>(blockIdx.x) * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
     grid_dep_wait();
     grid_dep_launch();
     if (r >= rows) return;  // whole warps only: a block-per-row launch has exactly `rows` blocks
@@ -157,6 +158,64 @@ __global__ void __launch_bounds__(kRowThreads)
     }
 }
 
+// The quantiser of bf16 rows, a warp each: the row waits for its maximum as it came, half the
+// registers of its fp32 values (71,550 x 2,048: 76 us with those, 65 so), and the maximum
+// is taken on the bits, which order like the values, infinities and NaN last.
+template <int CH>
+__global__ void __launch_bounds__(kWarpRowThreads)
+    bf16_rows_to_e4m3(const __nv_bfloat16 *__restrict__ x, int64_t rows, int dim, uint8_t *__restrict__ q,
+                      float *__restrict__ scale)
+{
+    constexpr uint32_t inf = 0x7f80u;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * (kWarpRowThreads / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    grid_dep_wait();
+    grid_dep_launch();
+    if (r >= rows) return;
+    uint4 u[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * 32 + lane) * 8;
+        u[c] = col < dim ? *reinterpret_cast<const uint4 *>(x + r * dim + col) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(u[c].x & 0x7fff7fffu, u[c].y & 0x7fff7fffu),
+                                   __vmaxu2(u[c].z & 0x7fff7fffu, u[c].w & 0x7fff7fffu)));
+    uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+    if (m >= inf) {  // rare: the maximum without what is not finite, and NaN in its place
+        m = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if ((w[i] & inf) == inf) w[i] |= 0x7fffu;
+                else m = max(m, w[i] & 0x7fffu);
+                if ((w[i] & (inf << 16)) == inf << 16) w[i] |= 0x7fff0000u;
+                else m = max(m, (w[i] >> 16) & 0x7fffu);
+            }
+            u[c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+    }
+    const float amax = fmaxf(__uint_as_float(m << 16), kTinyAmax), inv = kE4m3Max / amax;
+    if (lane == 0) scale[r] = amax / kE4m3Max;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * 32 + lane) * 8;
+        float2 a = unpack_bf16x2(u[c].x), b = unpack_bf16x2(u[c].y), d = unpack_bf16x2(u[c].z), e = unpack_bf16x2(u[c].w);
+        mul_f32x2(a.x, a.y, inv, inv);
+        mul_f32x2(b.x, b.y, inv, inv);
+        mul_f32x2(d.x, d.y, inv, inv);
+        mul_f32x2(e.x, e.y, inv, inv);
+        if (col < dim)
+            *reinterpret_cast<uint2 *>(q + r * dim + col) =
+                make_uint2(pack_e4m3x4(a.x, a.y, b.x, b.y), pack_e4m3x4(d.x, d.y, e.x, e.y));
+    }
+}
+
 // Any width and alignment: a block per row, the row read again for each pass.
 template <class IT, bool NORM>
 __global__ void __launch_bounds__(kRowThreads)
@@ -207,11 +266,15 @@ struct RowArgs {
 template <class IT, bool NORM, bool BLOCK, int CH>
 cudaError_t go(const RowArgs &a, cudaStream_t s)
 {
-    constexpr int per = kRowThreads / 32;
+    constexpr int per = kWarpRowThreads / 32;
     const int64_t grid = BLOCK ? a.rows : (a.rows + per - 1) / per;
-    return launch_k(rows_to_e4m3<IT, NORM, BLOCK, CH>, dim3(static_cast<unsigned>(grid)), dim3(kRowThreads), 0, s,
-                    static_cast<const IT *>(a.x), a.h32, a.w, a.wadd, a.eps, a.rows, a.dim,
-                    static_cast<uint8_t *>(a.q), a.scale);
+    if constexpr (!NORM && !BLOCK && sizeof(IT) == 2)
+        return launch_k(bf16_rows_to_e4m3<CH>, dim3(static_cast<unsigned>(grid)), dim3(kWarpRowThreads), 0, s,
+                        static_cast<const IT *>(a.x), a.rows, a.dim, static_cast<uint8_t *>(a.q), a.scale);
+    else
+        return launch_k(rows_to_e4m3<IT, NORM, BLOCK, CH>, dim3(static_cast<unsigned>(grid)),
+                        dim3(BLOCK ? kRowThreads : kWarpRowThreads), 0, s, static_cast<const IT *>(a.x), a.h32, a.w, a.wadd,
+                        a.eps, a.rows, a.dim, static_cast<uint8_t *>(a.q), a.scale);
 }
 
 template <class IT, bool NORM>
