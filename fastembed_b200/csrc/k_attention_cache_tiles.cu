@@ -15,10 +15,10 @@
 //     softmax of step k.  (One 128-column slot per stream, where S had to wait for the previous
 //     PV, took 250 us on the case below that takes 224 us now.)
 //   K stays in 8 bits: S = Q K^T as kind::f8f6f4 with Q in two e4m3 parts, q = hi + lo.  A bf16
-//     has 8 significant bits and each part holds 4, so after a power-of-two scaling of the row
-//     (maximum in [128, 256)) the split is exact down to 2^-10 of the row's largest element and
-//     off by at most 2^-18 of it below.  Two 8-bit products cost what one f16 product does and
-//     the codes are multiplied as they lie in memory: nothing converts K.
+//     has 8 significant bits and each part holds 4: hi is the upper four, lo the rest.  After a
+//     power-of-two scaling of the row (maximum in [128, 256)) that is exact down to 2^-10 of the
+//     row's largest element and off by at most 2^-16 of it below.  Two 8-bit products cost what one
+//     f16 product does and the codes are multiplied as they lie in memory: nothing converts K.
 //   V becomes f16 (exact) on four converter warps, which also zero the slots past the
 //     sequence's end; O += P V as kind::f16 with P (f16) in TMEM over S.
 //   Scales: an item's 16-token groups (a page holds at least one) each have (sk, log2 sv,
@@ -124,17 +124,12 @@ __host__ __device__ constexpr uint32_t idesc_f16_bt(int M, int N)
     return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
-// Two f16 values x (up to 256, 8 significant bits) as hi + lo: hi = e4m3(x), lo = e4m3(x - hi),
-// the difference exact in f16; NaN stays NaN.
-__device__ __forceinline__ void split_e4m3x2(uint32_t x, uint32_t &hi, uint32_t &lo)
+// Two bf16 times a power of two as e4m3 codes
+__device__ __forceinline__ uint32_t scaled_codes(uint32_t w, float f)
 {
-    uint16_t h, l;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
-    const uint32_t back = e4m3x2_to_f16x2(h);
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&back));
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(*reinterpret_cast<const uint32_t *>(&d)));
-    hi = h;
-    lo = l;
+    float2 x = unpack_bf16x2(w);
+    mul_f32x2(x.x, x.y, f, f);
+    return cvt_e4m3x2(x.x, x.y);
 }
 
 template <int HD>
@@ -465,9 +460,11 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2 x = unpack_bf16x2(w[j]);
-                        uint32_t h2, l2;
-                        split_e4m3x2(pack_f16x2(x.x * sign, x.y * sign), h2, l2);
+                        const uint32_t top = w[j] & 0xfff0fff0u;  // sign, exponent, three mantissa bits
+                        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&w[j]),
+                                                         *reinterpret_cast<const __nv_bfloat162 *>(&top));  // exact
+                        const uint32_t h2 = scaled_codes(top, sign);
+                        const uint32_t l2 = scaled_codes(*reinterpret_cast<const uint32_t *>(&d), sign);
                         h[j >> 1] = j & 1 ? h[j >> 1] | (h2 << 16) : h2;
                         l[j >> 1] = j & 1 ? l[j >> 1] | (l2 << 16) : l2;
                     }
@@ -582,36 +579,58 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         if (ok && steps > 0) ok = wait(&pv_done[slot_of(s, steps - 1)], phase_of(steps - 1));
         tc_fence_after();
         if (ok && warp_live) {
-            const int64_t orow = (static_cast<int64_t>(sq.t0) + token) * a.q_heads + head;
             const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // a row that sees nothing is zero
-            if (a.splits > 1 && live)
-                *reinterpret_cast<float2 *>(a.part_ml + (orow * a.splits + split) * 2) = make_float2(m_run, l_run);
+            if (a.splits > 1) {
+                const int64_t at = ((static_cast<int64_t>(sq.t0) + token) * a.q_heads + head) * a.splits + split;
+                if (live) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m_run, l_run);
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t v[32];
-                if (items > 0) {
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t v[32];
+                    if (items > 0) {
+                        tmem_ld_x32(tO + c, v);
+                        tmem_wait_ld_regs(v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0;
+                    }
+                    if (live) {
+                        float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * HD + c);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                                 __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                    }
+                    __syncwarp();
+                }
+            } else {
+                // Rows leave through this warp's share of Q's shared memory (every S that reads it is
+                // done), so that whole rows are stored side by side: a lane a row would be 32 lines
+                // an instruction.  16-byte chunks are permuted by the row against bank conflicts.
+                uint8_t *rowbuf = sQ + (s * 2 * C::KT) + q * (32 * HD * 2);
+                constexpr int CH = HD / 8;  // 16-byte chunks of a row
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t v[32];
                     tmem_ld_x32(tO + c, v);
                     tmem_wait_ld_regs(v);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = 0;
-                }
-                if (live && a.splits > 1) {
-                    float4 *dst = reinterpret_cast<float4 *>(a.part_o + (orow * a.splits + split) * HD + c);
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t o[4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        dst[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
-                                             __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
-                } else if (live) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(a.out + orow * HD + c);
-                    uint32_t o[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        o[i] = pack_bf16x2(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int j = 0; j < 4; ++j)
+                            o[j] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * j]) * inv, __uint_as_float(v[8 * i + 2 * j + 1]) * inv);
+                        *reinterpret_cast<uint4 *>(rowbuf + lane * (HD * 2) + (((c / 8 + i) ^ (lane & 7)) << 4)) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                    }
                 }
                 __syncwarp();
+                const int first = r0 + 128 * s + q * 32, count = min(32, rows - first);
+                for (int x = lane; x < count * CH; x += 32) {
+                    const int row = x / CH, ch = x % CH, tk = (first + row) / a.group;
+                    const int64_t orow = (static_cast<int64_t>(sq.t0) + tk) * a.q_heads + kvh * a.group + first + row - tk * a.group;
+                    *reinterpret_cast<uint4 *>(a.out + orow * HD + 8 * ch) =
+                        *reinterpret_cast<const uint4 *>(rowbuf + row * (HD * 2) + ((ch ^ (row & 7)) << 4));
+                }
             }
         }
     } else {
