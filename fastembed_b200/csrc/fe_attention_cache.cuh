@@ -1,4 +1,4 @@
-// fe_attention_cache.cuh — what the kernels of the attention over the paged 8-bit cache share:
+// fe_attention_cache.cuh — what the kernels of the paged 8-bit cache and its attention share:
 // arguments, the reading of a sequence's offsets, and the launcher of the tile kernel.
 #pragma once
 
@@ -21,6 +21,8 @@ struct CacheArgs {
     float scale_log2;
 };
 
+constexpr int kMaxCacheTokens = 1 << 30;  // of a sequence: token indexes fit 32 bits with room
+
 // One sequence of the batch: false (and a report) when its offsets do not describe it.
 struct CacheSeq {
     int t0, len, past, kv;  // first row, new tokens, tokens before them, tokens in the cache
@@ -34,7 +36,7 @@ __device__ __forceinline__ bool load_seq(const CacheArgs &a, int b, CacheSeq &s,
     s.len = t1 - s.t0;
     if (s.len <= 0) return false;
     const int64_t kv = static_cast<int64_t>(s.past) + s.len;
-    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 &&
+    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 && kv <= kMaxCacheTokens &&
                     kv <= (static_cast<int64_t>(a.width) << a.page_log2);
     s.kv = static_cast<int>(kv);
     if (!ok && threadIdx.x == 0) report(status, DEV_BAD_INPUT);

@@ -17,8 +17,7 @@
 // read once into registers (16 bytes a thread, hd / 8 threads a token), the block maximum
 // decides the scale, codes go out 8 bytes a thread.  Bound by HBM for prompts (2 bytes in, 1
 // out per element) and by latency (table -> rows -> codes) for single tokens.
-#include "fe_e4m3.cuh"
-#include "fe_internal.h"
+#include "fe_attention_cache.cuh"
 
 namespace fe {
 namespace {
@@ -97,7 +96,7 @@ struct AppendArgs {
     uint8_t *k, *v;
     float *ks, *vs;
     int64_t total, row;  // tokens and elements per row of qkv
-    int batch, width, pages, page, kv_heads, k_col0, v_col0;
+    int batch, max_len, width, pages, page, kv_heads, k_col0, v_col0;
 };
 
 // THREADS threads hold CH 16-byte chunks of K and of V each: CH * THREADS * 8 >= page * HD.
@@ -111,15 +110,15 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
     grid_dep_launch();
     const int t0 = a.cu[b], t1 = a.cu[b + 1], past = a.past[b];
     if (t1 <= t0) return;
-    if (t0 < 0 || t1 > a.total || past < 0) {  // offsets that do not describe the batch: nothing is touched
+    const int64_t end = static_cast<int64_t>(past) + t1 - t0;
+    if (t0 < 0 || t1 > a.total || t1 - t0 > a.max_len || past < 0 || end > kMaxCacheTokens ||
+        end > static_cast<int64_t>(a.width) * a.page) {  // offsets that do not describe the batch: nothing is touched
         if (threadIdx.x == 0) report(status, DEV_BAD_INPUT);
         return;
     }
-    const int64_t end = static_cast<int64_t>(past) + (t1 - t0);
     const int64_t ordinal = past / a.page + nth;
     const int64_t base = ordinal * a.page;  // first token of the page
     if (base >= end) return;
-    if (nth == reach - 1 && base + a.page < end && threadIdx.x == 0) report(status, DEV_BAD_INPUT);  // longer than max_len
     const int lo = past > base ? static_cast<int>(past - base) : 0;              // first new slot
     const int hi = end - base < a.page ? static_cast<int>(end - base) : a.page;  // past the last
 
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
             vr[c] = *reinterpret_cast<const uint4 *>(p + a.v_col0);
         }
     }
-    const int id = ordinal < a.width ? a.table[static_cast<int64_t>(b) * a.width + ordinal] : -1;
+    const int id = a.table[static_cast<int64_t>(b) * a.width + ordinal];
     if (id < 0 || id >= a.pages) {
         if (threadIdx.x == 0) report(status, DEV_BAD_INPUT);
         return;
@@ -196,9 +195,9 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
 }
 
 template <int HD>
-cudaError_t append(const AppendArgs &a, int max_len, cudaStream_t s)
+cudaError_t append(const AppendArgs &a, cudaStream_t s)
 {
-    const int reach = (a.page - 1 + max_len - 1) / a.page + 1;  // pages that max_len tokens at any offset can touch
+    const int reach = (a.page - 1 + a.max_len - 1) / a.page + 1;  // pages that max_len tokens at any offset can touch
     const dim3 grid(static_cast<unsigned>(a.batch) * reach, a.kv_heads);
     int *status = current_device_status_word();
     const int chunks = a.page * HD / 8;  // 128 (page 16, head_dim 64) to 4096 (128, 256)
@@ -224,12 +223,12 @@ cudaError_t launch_kv_cache_append_e4m3(const void *qkv, const int32_t *cu, int 
     a.ks = ks, a.vs = vs;
     a.total = total;
     a.row = static_cast<int64_t>(q_heads + 2 * kv_heads) * head_dim;
-    a.batch = batch, a.width = width, a.pages = pages, a.page = page, a.kv_heads = kv_heads;
+    a.batch = batch, a.max_len = max_len, a.width = width, a.pages = pages, a.page = page, a.kv_heads = kv_heads;
     a.k_col0 = q_heads * head_dim;
     a.v_col0 = (q_heads + kv_heads) * head_dim;
-    if (head_dim == 64) return append<64>(a, max_len, s);
-    if (head_dim == 128) return append<128>(a, max_len, s);
-    return append<256>(a, max_len, s);
+    if (head_dim == 64) return append<64>(a, s);
+    if (head_dim == 128) return append<128>(a, s);
+    return append<256>(a, s);
 }
 
 }  // namespace fe

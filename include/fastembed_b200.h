@@ -313,7 +313,8 @@ fe_status fe_quantize_rows_e4m3(const void *x, fe_dtype x_dtype, int64_t rows, i
                                 fe_stream_t stream);
 /* h32 += y in place (y fp32 or bf16 [rows, dim]; NULL: no addition, h32 is not written), then
  * RMSNorm(h32) = h32 / sqrt(mean(h32^2) + eps) * w (1 + w when one_plus) as fe_quantize_rows_e4m3
- * of its rows, normalised in fp32. */
+ * of its rows.  Sum of squares and normalisation in fp32: a row whose sum of squares passes
+ * 3.4e38 normalises to 0. */
 fe_status fe_add_rmsnorm_e4m3(const void *y, fe_dtype y_dtype, float *h32, const float *w, int32_t one_plus, float eps,
                               int64_t rows, int32_t dim, void *q, float *scale, fe_stream_t stream);
 /* y[m,n] = epilogue(x_scale[i] * w_scale[j] * (x[m,k] . w[n,k]^T)) over e4m3 codes, one scale
@@ -332,8 +333,8 @@ fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, con
  * [total_tokens, (q_heads + 2 kv_heads) * head_dim], rows cu_seqlens[b] .. cu_seqlens[b+1] the
  * new tokens of sequence b (at most max_len), at positions past_lens[b] and up.  head_dim 64,
  * 128 or 256.  cu_seqlens, past_lens and page_table are read on the device: a sequence whose
- * offsets do not fit (rows past total_tokens, more than max_len or table_width pages of tokens,
- * a negative past) is left out, and so are the tokens of a page id outside [0, pages); either
+ * offsets do not fit (rows past total_tokens, more than max_len new tokens, more than
+ * table_width pages or 2^30 tokens in all, a negative past) is left out, and so are the tokens of a page id outside [0, pages); either
  * sets FE_ERR_INVALID_ARGUMENT in the device status word. */
 
 /* Writes the new tokens' keys and values into their pages.  The scale of a (page, head) is the

@@ -515,3 +515,173 @@ def test_steps_captured_in_a_graph_and_on_a_side_stream(cuda_dev):
         assert torch.equal(y, w)
     assert torch.equal(cache.k.view(torch.uint8), wcache.k.view(torch.uint8))
     ops.device_status(0)
+
+
+# ------------------------------------------------------------ both attention kernels at every size
+@pytest.mark.parametrize("new,past", ATTENDS)
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (16, 8)), (128, (10, 2)), (256, (3, 1))])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_cache_loose_bound(cuda_dev, new, past, page, hd, heads, causal):
+    """max_kv_len is a bound: one far above the lengths gives sequences parts of which most are
+    empty, and turns rows that few tokens are read for over to the tile kernel."""
+    from fastembed_b200 import ops
+    b = Batch(new, past, page, *heads, hd, cuda_dev, seed=sum(new) + hd)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    b.max_kv = 1 << 20
+    _attend(b, ops, cache, causal)
+
+
+MANY = [65, 0, 17, 128, 1, 33, 64, 300, 129, 2, 96, 256]
+
+
+@pytest.mark.parametrize("hd,heads", [(64, (8, 8)), (64, (6, 2)), (128, (16, 8)), (128, (10, 2)), (256, (6, 2)), (256, (4, 4))])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_cache_many_prompts(cuda_dev, hd, heads, page, causal):
+    """Enough row tiles that no sequence is split."""
+    from fastembed_b200 import ops
+    b = Batch(MANY, [(37 * i * i) % 400 for i in range(len(MANY))], page, *heads, hd, cuda_dev, seed=hd + page, extra_rows=2)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    _attend(b, ops, cache, causal)
+
+
+@pytest.mark.parametrize("hd,heads,batch", [(128, (4, 2), 150), (64, (2, 2), 250), (256, (2, 1), 300), (128, (8, 1), 160)])
+@pytest.mark.parametrize("top", [1, 5])
+def test_attention_cache_many_sequences(cuda_dev, hd, heads, batch, top):
+    """Few rows each in more sequences than there are multiprocessors: one part each, or two."""
+    from fastembed_b200 import ops
+    b = Batch([(7 * i) % top + 1 for i in range(batch)], [(53 * i) % 700 for i in range(batch)], 32, *heads, hd, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    _attend(b, ops, cache)
+
+
+# ------------------------------------------------------------ lengths that do not fit, graphs, waits
+@pytest.mark.parametrize("new,bound", [([1, 6, 2], 300), ([1, 90, 2], 1 << 20), ([1, 6, 2], 1 << 20)])
+def test_longer_than_max_len_is_reported(cuda_dev, new, bound):
+    """A sequence with more new tokens than max_len: neither written, nor answered, nor read past; the
+    others as without it."""
+    from fastembed_b200 import ops
+    from fastembed_b200.capi import FeError
+    b = Batch(new, [20, 33, 40], 32, 8, 2, 128, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    ops.device_status(0)
+    short = new[1] - 1
+    state = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    out = torch.full((sum(new), 8 * 128), 3.0, dtype=torch.bfloat16, device=cuda_dev)
+    ops.attention_cache_e4m3(b.qkv, b.cu, short, b.past_lens, bound, b.table, cache, 8, out=out)
+    with pytest.raises(FeError):
+        ops.device_status(0)
+    want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, b.past, b.table, 8, True, 128 ** -0.5)
+    fits = (out.double() - want).abs() <= ref.attention_bound(want, mag, dot, floor, 128)
+    a, c = new[0], new[0] + new[1]
+    assert torch.all(out[a:c] == 3.0) and torch.all(fits[:a]) and torch.all(fits[c:])
+    b.qkv.neg_()
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, short, b.past_lens, b.table, cache, 8)
+    with pytest.raises(FeError):
+        ops.device_status(0)
+    t = b.table.cpu()
+    mine = {int(t[1, o]) for o in range(33 // 32, (33 + new[1] - 1) // 32 + 1)}
+    for was, now in zip(state, (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)):
+        for p in mine:
+            assert torch.equal(was[p], now[p])
+    ops.device_status(0)
+
+
+@pytest.mark.parametrize("new,past,bound", [([1, 1], [900, 300], 901), ([1, 1], [900, 300], 1 << 20),
+                                            ([70, 40], [600, 10], 1 << 20), (MANY, [5] * len(MANY), 400)])
+def test_attention_cache_captured(cuda_dev, new, past, bound):
+    """Each form of the attention (parts in a cluster, parts in a workspace, tiles in parts, tiles)
+    captured and replayed over changed queries and pages: the bits of eager calls.  Two graphs of one
+    stream with a workspace each."""
+    from fastembed_b200 import ops
+    b = Batch(new, past, 32, 16, 8, 128, cuda_dev, seed=5)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, 16)
+    run = lambda q: ops.attention_cache_e4m3(q, b.cu, b.max_new, b.past_lens, bound, b.table, cache, 16)
+    q1, q2 = b.qkv.clone(), (b.qkv.float() * -0.5).to(torch.bfloat16)
+    w1, w2 = run(q1), run(q2)
+    a1, a2 = torch.zeros_like(q1), torch.zeros_like(q2)
+    graphs, outs = [], []
+    for a in (a1, a2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(a))
+        graphs.append(g)
+    for src, dst in ((q1, a1), (q2, a2)):
+        dst.copy_(src)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], w1) and torch.equal(outs[1], w2)
+    a1.copy_(q2)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], w2)
+    ops.device_status(0)
+
+
+def _short_waits(call):
+    """The call under a wait limit of a microsecond, then under the default again: the status of the first, which
+    has the bits of a call before it unless it reports that a wait ran out, as the second has in any case."""
+    from fastembed_b200 import capi
+    L = capi.lib()
+    before = call().clone()
+    torch.cuda.synchronize()
+    assert L.fe_device_status(0) == 0
+    assert L.fe_set_wait_limit(0, 1000) == 0
+    try:
+        got = call()
+        st = L.fe_device_status(0)
+    finally:
+        assert L.fe_set_wait_limit(0, 2_000_000_000) == 0
+    assert st == 5 or (st == 0 and torch.equal(got, before)), st  # FE_ERR_DEVICE_TIMEOUT
+    assert torch.equal(call(), before)
+    torch.cuda.synchronize()
+    assert L.fe_device_status(0) == 0
+    return st
+
+
+@pytest.mark.parametrize("epi", ["none", "bias_residual"])
+def test_linear_wait_runs_out_then_recovers(cuda_dev, epi):
+    """One tile whose 64-block main loop takes tens of microseconds: the epilogue's wait for it runs out."""
+    from fastembed_b200 import ops
+    g = torch.Generator(device=cuda_dev).manual_seed(3)
+    x = ops.quantize_rows_e4m3(torch.randn(128, 8192, device=cuda_dev, generator=g))
+    w = ops.quantize_rows_e4m3(torch.randn(64, 8192, device=cuda_dev, generator=g))
+    bias, res = torch.randn(64, device=cuda_dev, generator=g), torch.randn(128, 64, device=cuda_dev, generator=g)
+    if epi == "none":
+        assert _short_waits(lambda: ops.linear_e4m3(*x, *w, None, None, "none", "f32")) == 5
+    else:
+        assert _short_waits(lambda: ops.linear_e4m3(*x, *w, bias, res, "bias_residual", "f32")) == 5
+
+
+@pytest.mark.parametrize("hd,heads", [(64, (8, 4)), (128, (16, 8)), (256, (6, 2))])
+def test_attention_cache_short_waits(cuda_dev, hd, heads):
+    """The tile kernel's waits are for a load, a product or a softmax step, a microsecond or two: they may run
+    out or not (the limit is looked at every 256 tries), and the call stays sound either way."""
+    from fastembed_b200 import ops
+    b = Batch([300, 17, 129, 64], [700, 0, 3000, 10], 64, *heads, hd, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    _short_waits(lambda: ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.max_kv, b.table, cache, b.q_heads))
+
+
+@pytest.mark.parametrize("m,n", [(64, 64), (300, 520), (511, 256), (700, 512)])
+def test_linear_residual_in_place_every_kernel(cuda_dev, m, n):
+    from fastembed_b200 import capi, ops
+    g = torch.Generator(device=cuda_dev).manual_seed(m)
+    x = ops.quantize_rows_e4m3(torch.randn(m, 256, device=cuda_dev, generator=g))
+    w = ops.quantize_rows_e4m3(torch.randn(n, 256, device=cuda_dev, generator=g))
+    bias, res = torch.randn(n, device=cuda_dev, generator=g), torch.randn(m, n, device=cuda_dev, generator=g)
+    want = ops.linear_e4m3(*x, *w, bias, res, "bias_residual", "f32")
+    y = res.clone()
+    capi.call("fe_linear_e4m3", x[0].data_ptr(), x[1].data_ptr(), w[0].data_ptr(), w[1].data_ptr(), bias.data_ptr(),
+              y.data_ptr(), y.data_ptr(), m, n, 256, capi.EPI["bias_residual"], capi.DTYPE["f32"],
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(y, want)
