@@ -573,7 +573,9 @@ cudaError_t launch_join(const CacheArgs &a, int head_dim, int *status, cudaStrea
     return head_dim == 64 ? launch_join<64>(a, status, s) : head_dim == 128 ? launch_join<128>(a, status, s) : launch_join<256>(a, status, s);
 }
 
-constexpr int kStreamRows = 32;    // rows of a key-value head up to which the streaming kernel runs
+constexpr int kStreamRows = 32;    // rows of a key-value head up to which the streaming kernel runs at any size
+constexpr int kStreamCtas = 2 * kSms;            // ... and with more rows up to so many CTAs, one part each, which
+constexpr int64_t kStreamTokens = int64_t{1} << 18;  // read so many tokens together
 constexpr int kClusterParts = 8;   // portable cluster size
 constexpr int kPartTokens = 128;   // a part has a run for each of four warps
 
@@ -590,7 +592,14 @@ struct CachePlan {
 CachePlan plan_attention_cache(int batch, int max_len, int max_kv, int q_heads, int kv_heads, int head_dim)
 {
     const int64_t rows = static_cast<int64_t>(max_len) * (q_heads / kv_heads);
-    CachePlan p{rows > kStreamRows, false, false, 1};
+    const int per = 8 * row_tile_count(rows, head_dim);
+    const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
+    // The streaming kernel reads the cache once per 8 or 16 rows, the tiles once per 128 or 256, but a tile
+    // CTA costs 7 to 25 us before its matrix products fill.  Streamed against tiles, heads 16 to 8 of 128:
+    // 1 sequence of 4,000 tokens, 30 new ones, 19 and 27 us, 60 new ones (64 CTAs, 260,000 tokens) 25 and 29;
+    // 8 of 500, 30 new ones (256 CTAs), 16 and 21; past the limits 4 of 4,000, 20 new ones, 40 and 34,
+    // 16 prompts of 30 (512 CTAs) 14 and 11.
+    CachePlan p{rows > kStreamRows && (ctas > kStreamCtas || ctas * max_kv > kStreamTokens), false, false, 1};
     if (p.tiles) {
         const int64_t tiles = (rows + attention_cache_tile_rows(head_dim) - 1) / attention_cache_tile_rows(head_dim);
         // one CTA an SM: split until they have one each, 512 tokens or more a part
@@ -598,14 +607,14 @@ CachePlan plan_attention_cache(int batch, int max_len, int max_kv, int q_heads, 
         p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
         return p;
     }
-    const int per = 8 * row_tile_count(rows, head_dim);
-    const int64_t ctas = std::max<int64_t>(1, (rows + per - 1) / per * batch * kv_heads);
-    constexpr int64_t resident = 3 * kSms;
-    if (ctas < resident && max_kv <= 2048 * std::min<int64_t>(resident / ctas, kClusterParts)) {
-        // As many parts as all fit at once, and those short.  (Beside more CTAs than that clusters wait for room: 7 parts of
-        // 32 sequences x 8 heads took 186 us as clusters and 158 with the second launch, one sequence of
-        // 2,000 tokens 8.5 and 14.9.)
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({resident / ctas, kClusterParts, max_kv / kPartTokens})));
+    const int64_t resident = (head_dim == 128 && per == 16 ? 2 : 3) * kSms;  // what registers allow
+    const int64_t room = std::min<int64_t>(resident / ctas, kClusterParts);
+    if (room > 1 && max_kv <= 2048 * room) {
+        // As many parts as all fit at once, and those short; a power of two, since clusters of 3 or 6 leave SMs of
+        // their group idle.  (Clusters that do not fit wait for room: 7 parts of 32 sequences x 8 heads
+        // took 186 us as clusters and 158 with the second launch, one sequence of 2,000 tokens 8.5 and 14.9;
+        // 16 sequences of 500, 5 new tokens, 3 parts for 2 CTAs an SM 21.8 us, 2 parts 12.8.)
+        while (2 * p.splits <= std::min<int64_t>(room, max_kv / kPartTokens)) p.splits *= 2;
         p.cluster = p.splits > 1;
     }
     if (p.splits == 1) {
