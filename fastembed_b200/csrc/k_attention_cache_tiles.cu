@@ -178,12 +178,13 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     const int all = (end + TK - 1) / TK, per = (all + a.splits - 1) / a.splits;
     const int j0 = split * per;
     const int items = max(0, min(per, all - j0));
+    const int streams = r0 + 128 < rows ? NS : 1;  // with a row; the second takes no part without
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) mbar_init(&q_full[i], 4);
         for (int i = 0; i < KS; ++i) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], NS);
+            mbar_init(&k_empty[i], streams);
         }
         for (int i = 0; i < RS; ++i) {
             mbar_init(&r_full[i], 1);
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         }
         for (int i = 0; i < VS; ++i) {
             mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], NS);
+            mbar_init(&v_empty[i], streams);
         }
         for (int i = 0; i < kEnt; ++i) mbar_init(&e_full[i], 1);
         for (int i = 0; i < 2 * NS; ++i) {
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         *abort_flag = 1;
         return false;
     };
+    auto given_up = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag != 0); };
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 }
             }
         };
-        for (int n = 0; n < items && ok && !*abort_flag; ++n) {
+        for (int n = 0; n < items && ok && !given_up(); ++n) {
             const int ks = n % KS, rs = n % RS;
             const int64_t row = lane < 8 ? page_row(j0 + n, lane) : none;
             float4 e = make_float4(0.f, -INFINITY, 0.f, 0.f);  // a group that is not there: weight 0
@@ -307,12 +309,6 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         constexpr uint32_t kt = C::KT >> 4, vt = C::VT >> 4;  // in descriptor units of 16 bytes
         constexpr uint32_t half_k = (HD == 64 ? 64 * 64 : 64 * 128) >> 4, half_v = 64 * 128 >> 4, box = TK * 128 >> 4;
         constexpr uint32_t hi_k = HD == 64 ? desc_hi(512, 4) : desc_hi(1024, 2), hi_v = desc_hi(1024, 2);
-        auto wait_lane = [&](uint64_t *bar, uint32_t parity) -> bool {
-            if (mbar_wait(bar, parity)) return true;
-            report(status, DEV_TIMEOUT);
-            *abort_flag = 1;
-            return false;
-        };
         bool issued = false;
         const uint32_t qs = desc_lo(smem_u32(sQ) + s * 2 * C::KT, 16), kd0 = desc_lo(smem_u32(sK), 16);
         const uint32_t vd0 = desc_lo(smem_u32(sV), TK * 128);  // MN-major: LBO between 64-column boxes
@@ -331,10 +327,10 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         // left: tokens from the step's first on (more than 0); par: the phase of the step's item
         auto issue_s = [&](auto hc, bool first, uint32_t par, int left) -> bool {
             constexpr int h = decltype(hc)::value;
-            if (h == 0 && !wait_lane(&k_full[kr.slot], kr.phase)) return false;
+            if (h == 0 && !wait(&k_full[kr.slot], kr.phase)) return false;
             if (first) {
-                if (h == 0 && !wait_lane(&q_full[s], 0)) return false;
-            } else if (!wait_lane(&pv_done[2 * s + h], par ^ 1)) {  // P of the slot's previous step consumed
+                if (h == 0 && !wait(&q_full[s], 0)) return false;
+            } else if (!wait(&pv_done[2 * s + h], par ^ 1)) {  // P of the slot's previous step consumed
                 return false;
             }
             tc_fence_after();
@@ -358,8 +354,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         };
         auto issue_pv = [&](auto hc, bool first, uint32_t par, int left) -> bool {
             constexpr int h = decltype(hc)::value;
-            if (h == 0 && !wait_lane(&v_full[vr.slot], vr.phase)) return false;
-            if (!wait_lane(&p_full[2 * s + h], par)) return false;
+            if (h == 0 && !wait(&v_full[vr.slot], vr.phase)) return false;
+            if (!wait(&p_full[2 * s + h], par)) return false;
             tc_fence_after();
             const uint32_t vd = vd0 + vr.at + h * half_v, pt = st + 64 * h;  // 16 tokens = 16 rows of 128 bytes
             if (leader) {
@@ -381,8 +377,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         constexpr std::integral_constant<int, 1> c1{};
         int left = min(end - j0 * TK, items * TK);  // tokens of this CTA's part from this item's first on
         uint32_t par = 0;
-        bool ok = items > 0 && issue_s(c0, true, 0, left) && (left <= 64 || issue_s(c1, true, 0, left - 64));
-        for (int n = 0; n < items && ok && !*abort_flag; ++n, left -= TK, par ^= 1) {
+        bool ok = items > 0 && s < streams && issue_s(c0, true, 0, left) && (left <= 64 || issue_s(c1, true, 0, left - 64));
+        for (int n = 0; n < items && ok && !given_up(); ++n, left -= TK, par ^= 1) {
             const bool first = n == 0;
             ok = issue_pv(c0, first, par, left) && (left <= TK || issue_s(c0, false, par ^ 1, left - TK));
             if (left > 64)
@@ -401,9 +397,9 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         const bool live = rr < rows, warp_live = r0 + 128 * s + q * 32 < rows;
         const int token = live ? rr / a.group : 0, head = kvh * a.group + (live ? rr - token * a.group : 0);
         const int vis = !live ? 0 : a.causal ? sq.past + token + 1 : sq.kv;  // tokens this row sees
-        bool ok = true;
+        bool ok = s < streams;
         float qf = 0.f;
-        {
+        if (ok) {
             // Q: the row's maximum to [128, 256), split in two e4m3 parts.  HD / 16 lanes share a row (16
             // values each), RPI rows at a time, the loads of up to eight such rounds in flight together.
             constexpr int LPR = HD / 16, RPI = 32 / LPR, IT = 32 / RPI < 8 ? 32 / RPI : 8;
@@ -479,24 +475,29 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         }
         const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
         const uint32_t tO = tmem + lanes + 256 + s * HD;
+        const int vis_all = __reduce_min_sync(0xffffffffu, vis);  // what every row of the warp sees
         float m_run = -INFINITY, l_run = 0.f;
+        bool spread = false;
         for (int k = 0; k < steps && ok; ++k) {  // 64 tokens at a time, from registers
             const int n = k >> 1, h = k & 1, c0 = 64 * h;
             const uint32_t tS = tmem + lanes + s * 128 + 64 * h;
-            if (h == 0 && !(ok = wait(&e_full[n % kEnt], (n / kEnt) & 1))) break;
+            if (h == 0) {
+                if (!(ok = wait(&e_full[n % kEnt], (n / kEnt) & 1))) break;
+                spread = ent[(n % kEnt) * 8].w != 0.f;
+            }
             if (!(ok = wait(&s_full[slot_of(s, k)], phase_of(k)))) break;
             tc_fence_after();
             const float4 *en = ent + (n % kEnt) * 8 + (c0 >> 4);
             const int lim = vis - (j0 + n) * TK - c0;  // columns of the step that the row sees
-            const bool spread = ent[(n % kEnt) * 8].w != 0.f;
             float alpha = 1.f;
+            bool raised = false;  // by a row of the warp
             if (warp_live) {
                 uint32_t v[64];
                 tmem_ld_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(v));
                 tmem_ld_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
                 tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v));
                 tmem_wait_ld_regs(*reinterpret_cast<uint32_t(*)[32]>(v + 32));
-                if (!__all_sync(0xffffffffu, 64 <= lim)) {
+                if (vis_all - (j0 + n) * TK - c0 < 64) {  // some row of the warp sees less
 #pragma unroll
                     for (int i = 0; i < 64; ++i)
                         if (i >= lim) v[i] = 0xff800000u;  // -inf
@@ -520,7 +521,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                     top = fmaxf(top, fmaf(fmaxf(m0, m1), f[i4], g[i4]));
                 }
                 // the reference rises only when a step exceeds it by more than 2^8
-                if (top > m_run + kLazy || m_run == -INFINITY) {
+                raised = __any_sync(0xffffffffu, top > m_run + kLazy || m_run == -INFINITY);
+                if (raised && (top > m_run + kLazy || m_run == -INFINITY)) {
                     top = fmaxf(top, m_run);
                     alpha = m_run == -INFINITY ? 0.f : exp2_fast(m_run - top);
                     m_run = top;
@@ -557,8 +559,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 tmem_wait_st();
             }
             // O *= alpha after the previous step's PV and before this one's
-            const bool rescale = k > 0 && warp_live && __any_sync(0xffffffffu, alpha != 1.f);
-            if (rescale) {
+            if (raised && k > 0) {
                 if (!(ok = wait(&pv_done[slot_of(s, k - 1)], phase_of(k - 1)))) break;
                 tc_fence_after();
 #pragma unroll 1
@@ -637,7 +638,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         // ------------------------------------------------ V converters
         const int t = threadIdx.x - 32 * (1 + NS + C::SOFT);
         constexpr int CPR = HD / 16;  // 16-code chunks per row
-        for (int n = 0; n < items && !*abort_flag; ++n) {
+        for (int n = 0; n < items && !given_up(); ++n) {
             const int rs = n % RS, vs = n % VS;
             if (!wait(&r_full[rs], (n / RS) & 1)) break;
             if (!wait(&v_empty[vs], ((n / VS) & 1) ^ 1)) break;

@@ -63,6 +63,25 @@ __device__ __forceinline__ void umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc
         : "memory");
 }
 
+// Commit of the pair's MMAs arriving at the leader (rank 0) alone.
+__device__ __forceinline__ void umma_commit_pair_leader(uint64_t *bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(1))
+        : "memory");
+}
+
+// A whole warp's wait: its lanes go on, or give up, together.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// A warp leaves its loop as one, whichever of its lanes read the flag before it was set
+__device__ __forceinline__ bool given_up(const volatile int *flag) { return __any_sync(0xffffffffu, *flag != 0); }
+
 struct EpiArgs {
     const float *sx;        // [M]
     const float *sw;        // [N]
@@ -262,7 +281,7 @@ __device__ __forceinline__ bool drain_residual(uint32_t t_row, int store_row, in
         float z[32];
         scale_bias(z, v, sx, sl.cols + c, sl.cols + COLS + c);
         const int slab = sl.pp;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sl.bar[slab], (sl.phase >> slab) & 1u))) {
+        if (!warp_wait(&sl.bar[slab], (sl.phase >> slab) & 1u)) {
             tmem_wait_ld();
             return false;
         }
@@ -297,7 +316,7 @@ __device__ __forceinline__ bool finish_tile(uint64_t *acc_full, uint32_t parity,
     if (any) stage_cols<COLS>(sl.cols, ea.sw, ea.epi == E_NONE ? nullptr : ea.bias, n0, N, lane);
     if constexpr (!OUT_BF16)
         if (ea.epi == E_RESID && any) start_residual<COLS>(tm_r, sl, n0, store_row, lane);
-    if (!__all_sync(0xffffffffu, mbar_wait(acc_full, parity))) return false;
+    if (!warp_wait(acc_full, parity)) return false;
     tc_fence_after();
     if (!any) return true;
     if constexpr (OUT_BF16) {
@@ -357,7 +376,8 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
     uint64_t *acc_full = empty + C::STAGES;  // [2]
     uint64_t *acc_empty = acc_full + 2;      // [2]
     uint64_t *res_bar = acc_empty + 2;       // [EPI_WARPS][2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_bar + 2 * C::EPI_WARPS);
+    uint64_t *probe = res_bar + 2 * C::EPI_WARPS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(probe + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
@@ -376,6 +396,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
             mbar_init(&acc_empty[b], C::EPI_WARPS);
         }
         for (int b = 0; b < 2 * C::EPI_WARPS; ++b) mbar_init(&res_bar[b], 1);
+        mbar_init(probe, 1);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_x);
@@ -427,8 +448,8 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool issued = false;
-        for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x) {
-            if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1)) {
+        for (int tile = blockIdx.x; tile < num_tiles && !given_up(abort_flag); tile += gridDim.x) {
+            if (!warp_wait(&acc_empty[acc], acc_phase ^ 1)) {
                 report(status, DEV_TIMEOUT);
                 *abort_flag = 1;
                 break;
@@ -436,7 +457,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * BN;
             for (int kb = 0; kb < k_iters; ++kb) {
-                if (!mbar_wait(&full[stage], phase)) {
+                if (!warp_wait(&full[stage], phase)) {
                     report(status, DEV_TIMEOUT);
                     *abort_flag = 1;
                     break;
@@ -454,14 +475,14 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
                     phase ^= 1;
                 }
             }
-            if (*abort_flag) break;
+            if (given_up(abort_flag)) break;
             if (leader) umma_commit(&acc_full[acc]);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
         }
-        if (*abort_flag && issued) {  // outstanding MMAs retire before TMEM is released
-            if (leader) umma_commit(&acc_full[acc]);
-            if (!mbar_wait_drain(&acc_full[acc], acc_phase)) report(status, DEV_TIMEOUT);
+        if (issued) {  // MMAs retire before TMEM is released, also where the epilogue gave up on them
+            if (leader) umma_commit(probe);
+            if (!mbar_wait_drain(probe, 0)) report(status, DEV_TIMEOUT);
         }
     } else {
         const int q = warp & 3;  // TMEM lane quarter this warp may access
@@ -469,7 +490,7 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
-            if (*abort_flag) break;
+            if (given_up(abort_flag)) break;
             const int m0 = tile / n_tiles * 128 + q * 32, n0 = tile % n_tiles * BN;
             const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
             if (!finish_tile<BN, OUT_BF16>(&acc_full[acc], acc_phase, t_row, m0 + lane, m0, n0, M, N, ea, &tm_y, &tm_r, sl,
@@ -532,7 +553,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
     uint64_t *acc_full = empty + C::STAGES;                           // both CTAs [2]
     uint64_t *acc_empty = acc_full + 2;                               // used in the leader [2]
     uint64_t *res_bar = acc_empty + 2;       // [EPI_WARPS][2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_bar + 2 * C::EPI_WARPS);
+    uint64_t *probe = res_bar + 2 * C::EPI_WARPS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(probe + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
@@ -554,6 +576,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             mbar_init(&acc_empty[b], 2 * C::EPI_WARPS);  // one arrival per epilogue warp of either CTA
         }
         for (int b = 0; b < 2 * C::EPI_WARPS; ++b) mbar_init(&res_bar[b], 1);
+        mbar_init(probe, 1);
         *abort_flag = 0;
         fence_mbar_init();
         tma_prefetch_desc(&tm_x);
@@ -611,8 +634,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool issued = false;
-            for (int tile = pair; tile < num_tiles && !*abort_flag; tile += npairs) {
-                if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1)) {
+            for (int tile = pair; tile < num_tiles && !given_up(abort_flag); tile += npairs) {
+                if (!warp_wait(&acc_empty[acc], acc_phase ^ 1)) {
                     report(status, DEV_TIMEOUT);
                     *abort_flag = 1;
                     break;
@@ -620,7 +643,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * C::BN;
                 for (int kb = 0; kb < k_iters; ++kb) {
-                    if (!mbar_wait(&full[stage], phase)) {
+                    if (!warp_wait(&full[stage], phase)) {
                         report(status, DEV_TIMEOUT);
                         *abort_flag = 1;
                         break;
@@ -638,14 +661,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
                         phase ^= 1;
                     }
                 }
-                if (*abort_flag) break;
+                if (given_up(abort_flag)) break;
                 if (leader) umma_commit_pair_both(&acc_full[acc]);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1;
             }
-            if (*abort_flag && issued) {
-                if (leader) umma_commit_pair_both(&acc_full[acc]);
-                if (!mbar_wait_drain(&acc_full[acc], acc_phase)) report(status, DEV_TIMEOUT);
+            if (issued) {  // as above
+                if (leader) umma_commit_pair_leader(probe);
+                if (!mbar_wait_drain(probe, 0)) report(status, DEV_TIMEOUT);
             }
         }
     } else {
@@ -656,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = pair; tile < num_tiles; tile += npairs) {
-            if (*abort_flag) break;
+            if (given_up(abort_flag)) break;
             const int m0 = tile / n_tiles * 256 + static_cast<int>(rank) * 128 + q * 32;
             const int n0 = tile % n_tiles * C::BN + h * C::COLS;
             const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * C::BN + h * C::COLS;
