@@ -192,8 +192,9 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 x = unpack_bf16x2(w[i]);
-                        f[j][8 * h + 2 * i] = x.x;
-                        f[j][8 * h + 2 * i + 1] = x.y;
+                        // an infinity becomes NaN (0 * inf): its products could all be -inf, a row that sees nothing
+                        f[j][8 * h + 2 * i] = fmaf(x.x, 0.f, x.x);
+                        f[j][8 * h + 2 * i + 1] = fmaf(x.y, 0.f, x.y);
                         m = fmaxf(m, fmaxf(finite_abs(x.x), finite_abs(x.y)));
                     }
                 }

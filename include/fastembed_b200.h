@@ -342,8 +342,8 @@ fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, con
  * page so far (0 if all are zero); when new tokens raise it, the page's older codes are
  * re-encoded.  The page of slot 0 starts afresh, whatever it held.  A token with a non-finite
  * key or value element of a head stores NaN as all of that key (and 0 for such value elements):
- * queries that see it get NaN.  A page that two sequences share may be read by both but must
- * not be reached by new tokens of more than one of them in one call. */
+ * queries that see it get NaN.  A page that two sequences share may be read by both; new tokens
+ * of one call must reach a page by one entry of page_table only. */
 fe_status fe_kv_cache_append_e4m3(const void *qkv, const int32_t *cu_seqlens, int32_t batch, int32_t max_len,
                                   int64_t total_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                   const int32_t *past_lens, const int32_t *page_table, int32_t table_width, void *k_pages,
@@ -358,7 +358,8 @@ fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int
  * past_lens[b] + len of them.  Query head h reads key-value head h / (q_heads / kv_heads).
  * max_kv_len is the caller's bound on past_lens[b] + len: it decides how sequences are split
  * over CTAs, not what is read.  Rows of out that belong to no sequence are left as they are; a
- * row that sees nothing (its pages are all out of range) is zero.  Scales may be any finite
+ * row that sees nothing (its pages are all out of range) is zero, one with a non-finite query
+ * element that sees a token NaN, as is one whose logits pass fp32.  Scales may be any finite
  * positive numbers or 0; value codes of visible tokens must not be NaN (append writes none).
  * Weights are f16 relative to the row's largest (weights times value scales): 11 bits each, and
  * 2^-32 of the largest at the least; sums are fp32.

@@ -685,3 +685,78 @@ def test_linear_residual_in_place_every_kernel(cuda_dev, m, n):
               y.data_ptr(), y.data_ptr(), m, n, 256, capi.EPI["bias_residual"], capi.DTYPE["f32"],
               torch.cuda.current_stream().cuda_stream)
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+@pytest.mark.parametrize("bound", [200, 1 << 20])
+def test_attention_cache_non_finite_queries(cuda_dev, hd, heads, bound):
+    """An infinity or NaN among a query's elements: that head's row is NaN whatever the keys' signs
+    are, the others as without it.  By streaming and (300 new tokens, loose bound) by tiles."""
+    from fastembed_b200 import ops
+    b = Batch([3, 300 if bound > 1000 else 12], [90, 33], 32, *heads, hd, cuda_dev)
+    b.qkv.view(-1, heads[0] + 2 * heads[1], hd)[:, heads[0]:, 1] = 1.0  # keys (and values) of one sign there
+    cache = b.random_cache(ops)
+    cache.k[..., 1] = torch.tensor(200.0, device=cuda_dev).to(F8)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    run = lambda: ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound, b.table, cache, b.q_heads)
+    want = run().view(-1, heads[0], hd).clone()
+    q = b.qkv.view(-1, heads[0] + 2 * heads[1], hd)
+    spots = [(0, 0, math.inf), (2, 1, -math.inf), (4, 0, -math.inf), (7, 2, math.nan), (14, 1, math.inf)]
+    for t, h, x in spots:
+        q[t, h, 1] = x
+    got = run().view(-1, heads[0], hd)
+    for t, h, x in spots:
+        assert torch.isnan(got[t, h]).all(), (t, h, x)
+        got[t, h] = want[t, h]
+    assert torch.equal(got, want)
+    ops.device_status(0)
+
+
+def test_front_end_refuses(cuda_dev):
+    """What the front end turns away before a launch, and what the library does."""
+    from fastembed_b200 import ops
+    from fastembed_b200.capi import FeError
+    b = Batch([2, 1], [5, 9], 16, 4, 2, 64, cuda_dev)
+    cache = b.random_cache(ops)
+    calls = {"append": lambda **k: ops.kv_cache_append_e4m3(*[k.get(n, v) for n, v in base.items()]),
+             "attend": lambda **k: ops.attention_cache_e4m3(
+                 *[k.get(n, v) for n, v in list(base.items())[:4]], 20, *[k.get(n, v) for n, v in list(base.items())[4:]],
+                 out=k.get("out"))}
+    base = dict(qkv=b.qkv, cu=b.cu, max_len=2, past=b.past_lens, table=b.table, cache=cache, q_heads=4)
+    bad = [dict(qkv=b.qkv.float()), dict(qkv=b.qkv[:, :-64]), dict(qkv=b.qkv.cpu()), dict(qkv=b.qkv.t()), dict(cu=b.cu.long()),
+           dict(cu=b.cu[:2]), dict(past=b.past_lens[:1]), dict(past=b.past_lens.cpu()), dict(table=b.table[:1]),
+           dict(table=b.table.float()), dict(cache=cache._replace(v=cache.v[1:])), dict(cache=cache._replace(k=cache.k[0])),
+           dict(cache=cache._replace(k_scale=cache.k_scale.half())), dict(cache=cache._replace(v=cache.v.view(torch.uint8)))]
+    for name, call in calls.items():
+        for kw in bad:
+            with pytest.raises(ValueError):
+                call(**kw)
+        with pytest.raises((ValueError, FeError)):
+            call(q_heads=3)
+        with pytest.raises(FeError):
+            call(max_len=-1)
+        odd = torch.zeros(b.qkv.numel() + 1, dtype=torch.bfloat16, device=cuda_dev)[1:].view(b.qkv.shape)
+        with pytest.raises(FeError):
+            call(qkv=odd)
+    with pytest.raises(ValueError):
+        calls["attend"](out=torch.zeros(3, 256, device=cuda_dev))
+    x, s = ops.quantize_rows_e4m3(torch.randn(4, 64, device=cuda_dev))
+    w, ws = ops.quantize_rows_e4m3(torch.randn(64, 64, device=cuda_dev))
+    one = torch.ones(64, device=cuda_dev)
+    for args in ((x, s[:3], w, ws), (x, s, w[:, :32], ws), (x, s, w, ws[:5]), (x.view(torch.uint8), s, w, ws), (x, s, w, ws, one[:8]),
+                 (x, s, w, ws, one, torch.zeros(4, 32, device=cuda_dev)), (x.t(), s, w, ws), (x[0], s, w, ws)):
+        with pytest.raises(ValueError):
+            ops.linear_e4m3(*args)
+    for kw in (dict(epilogue="bias"), dict(epilogue="swiglu"), dict(epilogue="bias_residual", out_dtype="f32", bias=one),
+               dict(epilogue="bias_gelu", bias=one, out_dtype="f32")):
+        with pytest.raises(FeError):
+            ops.linear_e4m3(x, s, w, ws, **kw)
+    for call in (lambda: ops.quantize_rows_e4m3(one.half()[None]), lambda: ops.quantize_rows_e4m3(one),
+                 lambda: ops.quantize_rows_e4m3(torch.ones(8, 8, device=cuda_dev).t()[1:]),
+                 lambda: ops.add_rmsnorm_e4m3(None, one[None], one[:8], 1e-6),
+                 lambda: ops.add_rmsnorm_e4m3(one.half()[None], one[None], one, 1e-6)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(FeError):
+        ops.add_rmsnorm_e4m3(None, one[None], one, -1.0)
+    ops.device_status(0)
