@@ -13,7 +13,7 @@
 //   Steps of 64 tokens: a stream has two 64-column S slots in TMEM, S of a step goes into the
 //     slot that the step before the last has left, and so S(k + 1) and PV(k - 1) run under the
 //     softmax of step k.  (One 128-column slot per stream, where S had to wait for the previous
-//     PV, took 250 us on the case below that takes 224 us now.)
+//     PV, took 250 us where this took 224: 8 prompts of 2,000 tokens after 1,000, 16 heads to 8, now 219.)
 //   K stays in 8 bits: S = Q K^T as kind::f8f6f4 with Q in two e4m3 parts, q = hi + lo.  A bf16
 //     has 8 significant bits and each part holds 4: hi is the upper four, lo the rest.  After a
 //     power-of-two scaling of the row (maximum in [128, 256)) that is exact down to 2^-10 of the
@@ -147,21 +147,19 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     uint8_t *sV = sR + RS * C::KT;              // [VS] f16 V, HD / 64 boxes of 128 rows x 128 bytes
     float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, 1 / sv, (group 0) spread flag
     uint64_t *bars = reinterpret_cast<uint64_t *>(ent + kEnt * 8);
-    uint64_t *q_full = bars;            // [NS] one arrival per softmax warp of the stream
-    uint64_t *k_full = q_full + NS;     // [KS]
+    uint64_t *k_full = bars;            // [KS]
     uint64_t *k_empty = k_full + KS;    // [KS] a commit per stream
     uint64_t *r_full = k_empty + KS;    // [RS]
     uint64_t *r_empty = r_full + RS;    // [RS] one arrival per converter warp
     uint64_t *v_full = r_empty + RS;    // [VS] one arrival per converter warp
     uint64_t *v_empty = v_full + VS;    // [VS] a commit per stream
-    uint64_t *e_full = v_empty + VS;    // [kEnt]
-    uint64_t *s_full = e_full + kEnt;     // [NS][slot]
+    uint64_t *s_full = v_empty + VS;      // [NS][slot]
     uint64_t *p_full = s_full + 2 * NS;   // [NS][slot] one arrival per softmax warp
     uint64_t *pv_done = p_full + 2 * NS;  // [NS][slot]
     uint64_t *probe = pv_done + 2 * NS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(probe + NS);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    static_assert((8 * NS + 2 * KS + 2 * RS + 2 * VS + kEnt) * 8 + 8 <= 512, "barrier space");
+    static_assert((7 * NS + 2 * KS + 2 * RS + 2 * VS) * 8 + 8 <= 512, "barrier space");
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -181,7 +179,6 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     const int streams = r0 + 128 < rows ? NS : 1;  // with a row; the second takes no part without
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) mbar_init(&q_full[i], 4);
         for (int i = 0; i < KS; ++i) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], streams);
@@ -194,7 +191,6 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
             mbar_init(&v_full[i], 4);
             mbar_init(&v_empty[i], streams);
         }
-        for (int i = 0; i < kEnt; ++i) mbar_init(&e_full[i], 1);
         for (int i = 0; i < 2 * NS; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
@@ -203,18 +199,21 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         for (int i = 0; i < NS; ++i) mbar_init(&probe[i], 1);
         *abort_flag = 0;
         fence_mbar_init();
-        tma_prefetch_desc(&tm_k);
-        tma_prefetch_desc(&tm_v);
+        fence_proxy_async_smem();
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    grid_dep_launch();
-    const uint32_t tmem = *tmem_slot;  // S slot k & 1 of stream s at 128 s + 64 (k & 1), O of stream s at 256 + s * HD
+    __syncwarp();
+    // Until here only warp 0 has anything of the CTA's state.  It starts the first item's loads while warp 1
+    // allocates TMEM and the softmax warps quantise Q; then all meet (that after a common set-up:
+    // 0.3 us more a unit of 7 in a row, 0.5 at head_dim 256).  S slot k & 1 of stream s is at
+    // TMEM column 128 s + 64 (k & 1), O of stream s at 256 + s HD.
+    auto meet = [&]() -> uint32_t {
+        tc_fence_before();
+        asm volatile("bar.sync 0;" ::: "memory");
+        tc_fence_after();
+        grid_dep_launch();
+        return *reinterpret_cast<volatile uint32_t *>(tmem_slot);
+    };
+    uint32_t tmem;
 
     // step k is half k & 1 of item k / 2; a step that lies past the end is not there
     const int steps = items == 0 ? 0 : 2 * items - (end - (j0 + items - 1) * TK <= 64 ? 1 : 0);
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 }
             }
         };
-        for (int n = 0; n < items && ok && !given_up(); ++n) {
+        auto fetch = [&](int n) -> bool {
             const int ks = n % KS, rs = n % RS;
             const int64_t row = lane < 8 ? page_row(j0 + n, lane) : none;
             float4 e = make_float4(0.f, -INFINITY, 0.f, 0.f);  // a group that is not there: weight 0
@@ -285,24 +284,32 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 have_ref = true;
             }
             spread |= __any_sync(0xffffffffu, row != none && fabsf(e.y - ref) > 30.f);
-            if (!(ok = wait(&k_empty[ks], ((n / KS) & 1) ^ 1))) break;
+            if (!wait(&k_empty[ks], ((n / KS) & 1) ^ 1)) return false;
             if (lane < 8) {
                 e.w = spread ? 1.f : 0.f;
                 ent[(n % kEnt) * 8 + lane] = e;
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&e_full[n % kEnt]);
+            __syncwarp();  // the entries are written before the leader's arrival for K
             load(&tm_k, sK + ks * C::KT, &k_full[ks], row);
             kn = n + 1;
-            if (!(ok = wait(&r_empty[rs], ((n / RS) & 1) ^ 1))) break;
+            if (!wait(&r_empty[rs], ((n / RS) & 1) ^ 1)) return false;
             load(&tm_v, sR + rs * C::KT, &r_full[rs], row);
             vn = n + 1;
-        }
+            return true;
+        };
+        if (items > 0) ok = fetch(0);
+        tmem = meet();
+        for (int n = 1; n < items && ok && !given_up(); ++n) ok = fetch(n);
         // every load this warp started lands before the CTA exits
         for (int n = max(0, kn - KS); n < kn; ++n) (void)mbar_wait_drain(&k_full[n % KS], (n / KS) & 1);
         for (int n = max(0, vn - RS); n < vn; ++n) (void)mbar_wait_drain(&r_full[n % RS], (n / RS) & 1);
     } else if (warp <= NS) {
         // ------------------------------------------------ MMA issuer of a stream
+        if (warp == 1) {
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        }
+        tmem = meet();
         const int s = warp - 1;
         const bool leader = elect_lane();
         constexpr uint32_t idesc_o = idesc_f16_bt(128, HD);
@@ -328,11 +335,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         auto issue_s = [&](auto hc, bool first, uint32_t par, int left) -> bool {
             constexpr int h = decltype(hc)::value;
             if (h == 0 && !wait(&k_full[kr.slot], kr.phase)) return false;
-            if (first) {
-                if (h == 0 && !wait(&q_full[s], 0)) return false;
-            } else if (!wait(&pv_done[2 * s + h], par ^ 1)) {  // P of the slot's previous step consumed
-                return false;
-            }
+            if (!first && !wait(&pv_done[2 * s + h], par ^ 1)) return false;  // P of the slot's previous step consumed
             tc_fence_after();
             const uint32_t idesc = idesc_f8(128, min(64, (left + 15) & ~15));
             const uint32_t kd = kd0 + kr.at + h * half_k;
@@ -470,9 +473,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 }
             }
             fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[s]);
         }
+        tmem = meet();
         const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
         const uint32_t tO = tmem + lanes + 256 + s * HD;
         const int vis_all = __reduce_min_sync(0xffffffffu, vis);  // what every row of the warp sees
@@ -481,12 +483,11 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         for (int k = 0; k < steps && ok; ++k) {  // 64 tokens at a time, from registers
             const int n = k >> 1, h = k & 1, c0 = 64 * h;
             const uint32_t tS = tmem + lanes + s * 128 + 64 * h;
-            if (h == 0) {
-                if (!(ok = wait(&e_full[n % kEnt], (n / kEnt) & 1))) break;
-                spread = ent[(n % kEnt) * 8].w != 0.f;
-            }
             if (!(ok = wait(&s_full[slot_of(s, k)], phase_of(k)))) break;
             tc_fence_after();
+            // The item's scales need no barrier of their own (226 us with one, 220 without): the producer wrote
+            // them before its arrival for K, which the issuer saw before it committed S.
+            if (h == 0) spread = ent[(n % kEnt) * 8].w != 0.f;
             const float4 *en = ent + (n % kEnt) * 8 + (c0 >> 4);
             const int lim = vis - (j0 + n) * TK - c0;  // columns of the step that the row sees
             float alpha = 1.f;
@@ -636,6 +637,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         }
     } else {
         // ------------------------------------------------ V converters
+        tmem = meet();
         const int t = threadIdx.x - 32 * (1 + NS + C::SOFT);
         constexpr int CPR = HD / 16;  // 16-code chunks per row
         for (int n = 0; n < items && !given_up(); ++n) {
