@@ -760,10 +760,16 @@ cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, co
     const bool glu = epilogue == E_SWIGLU || epilogue == E_GEGLU;
     const int64_t ny = glu ? n / 2 : n;
     const int sms = current_sm_count();
+    // The narrowest tiles of 64 and 128 columns that are one round of the SMs, else pairs; without the rows
+    // for those (or the columns), 256 columns where that is no more work per SM than 128.  At K =
+    // 4,096: 1,024 x 1,024 is 128 tiles of 64, 10.7 us (of 128 11.2, 16 pairs 15.6); 2,048 x 1,024 128 of
+    // 128, 12.1 (pairs 15.9, two rounds of 64 17.5); 4,099 x 1,024 68 pairs, 16.8 (two rounds of 128 19.4);
+    // 300 x 8,192 96 of 256, 16.7 (192 of 128 18.7); 300 x 16,384 384 of 128, 27.8 (192 of 256 34.0).
     auto tiles = [&](int64_t bn) { return (m + 127) / 128 * ((n + bn - 1) / bn); };
-    const bool pair = m >= 512 && n >= 256;
+    auto rounds = [&](int64_t bn) { return (tiles(bn) + sms - 1) / sms; };
+    const bool pair = m >= 512 && n >= 256 && tiles(128) > sms;
     // the gated epilogues pair 32 gate with 32 input columns and fill a slab from 128
-    const int bn = pair ? 128 : n > 128 && tiles(256) >= sms ? 256 : glu || tiles(128) >= sms ? 128 : 64;
+    const int bn = pair ? 128 : !glu && tiles(64) <= sms ? 64 : n > 128 && tiles(128) > sms && 2 * rounds(256) <= rounds(128) ? 256 : 128;
     Maps t;
     fe_status r = make_tmap_2d(&t.x, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, m, k, k, 128, BK);
     if (r == FE_OK) r = make_tmap_2d(&t.w, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, n, k, k, bn, BK);

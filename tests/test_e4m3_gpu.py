@@ -760,3 +760,37 @@ def test_front_end_refuses(cuda_dev):
     with pytest.raises(FeError):
         ops.add_rmsnorm_e4m3(None, one[None], one, -1.0)
     ops.device_status(0)
+
+
+# ------------------------------------------------------------ linear layers past one round of tiles
+@pytest.mark.parametrize("m,n,k", [(1030, 2312, 272), (2600, 1000, 48), (20000, 264, 128), (513, 5000, 400), (700, 4104, 1024),
+                                   (300, 16384, 144), (511, 8200, 160), (130, 30000, 80)])
+@pytest.mark.parametrize("epi,out", [("none", "bf16"), ("bias", "f32"), ("bias_residual", "f32"), ("bias_gelu", "bf16")])
+def test_linear_large(cuda_dev, m, n, k, epi, out):
+    """Pairs of CTAs, and tiles of 128 and 256 columns in several rounds, at ragged edges."""
+    test_linear(cuda_dev, m, n, k, epi, out)
+
+
+@pytest.mark.parametrize("m,n,k", [(1100, 2304, 272), (3000, 768, 768), (300, 16384, 144), (511, 8192, 160)])
+@pytest.mark.parametrize("epi", ["swiglu", "geglu"])
+def test_linear_gated_large(cuda_dev, m, n, k, epi):
+    test_linear_gated(cuda_dev, m, n, k, epi)
+
+
+def test_linear_rows_alone_across_kernels(cuda_dev):
+    """Rows of a call that pairs of CTAs compute, alone: the same bits from every tile size; in place too."""
+    from fastembed_b200 import capi, ops
+    g = torch.Generator(device=cuda_dev).manual_seed(8)
+    x, xs = _e4m3_rows(3001, 640, cuda_dev, g)
+    w, ws = _e4m3_rows(1032, 640, cuda_dev, g)
+    b = torch.randn(1032, device=cuda_dev, generator=g)
+    r = torch.randn(3001, 1032, device=cuda_dev, generator=g)
+    run = lambda lo, hi: ops.linear_e4m3(x[lo:hi].contiguous(), xs[lo:hi].contiguous(), w, ws, b, r[lo:hi].contiguous(),
+                                         "bias_residual", "f32")
+    whole = run(0, 3001)
+    for lo, hi in ((0, 1), (100, 1000), (5, 2100), (2999, 3001)):
+        assert torch.equal(run(lo, hi), whole[lo:hi])
+    capi.call("fe_linear_e4m3", x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), b.data_ptr(), r.data_ptr(),
+              r.data_ptr(), 3001, 1032, 640, capi.EPI["bias_residual"], capi.DTYPE["f32"],
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(r, whole)
