@@ -343,14 +343,23 @@ __device__ __forceinline__ void leave(Slabs &sl, int *status, int lane)
 }
 
 // ------------------------------------------------------------------ one CTA
+// Rows of x that a tile loads: of a single one only those there are (in eights); the MMA multiplies
+// whatever lies behind them, into rows that are not stored.  8 x 4,096 x 4,096 takes 8.9 us, with all
+// 128 rows loaded, most of them zeros from outside the tensor, 11.8.
+__host__ __device__ __forceinline__ int x_rows(int M) { return M < 128 ? (M + 7) & ~7 : 128; }
+
 template <int BN>
 struct CtaCfg {
     static constexpr int EPI_WARPS = 4;
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static constexpr int STAGES = BN == 256 ? 3 : BN == 128 ? 5 : 7;
+    static constexpr int STAGES = BN == 128 ? 5 : 3;
+    // Blocks of BK a stage.  One wait, commit and release each take longer than a block's four MMAs at 64
+    // columns: 8 x 1,024 x 4,096 takes 8.6 us with two blocks a stage, 9.6 with one (and seven stages).
+    static constexpr int GROUP = BN == 64 ? 2 : 1;
     static constexpr uint32_t A_BYTES = 128 * BK;
     static constexpr uint32_t B_BYTES = BN * BK;
-    static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
+    static constexpr uint32_t BLOCK = A_BYTES + B_BYTES;
+    static constexpr uint32_t STAGE = GROUP * BLOCK;
     static constexpr uint32_t RING = STAGES * STAGE;
     static constexpr uint32_t EPI = EPI_WARPS * 2 * kSlab;
     static constexpr uint32_t COLV = EPI_WARPS * 2 * BN * 4;  // column vectors
@@ -420,16 +429,21 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
             uint32_t phase = 0, armed = 0, armed_parity = 0;  // per stage: armed at least once / parity of the last arm
             for (int tile = blockIdx.x; tile < num_tiles && !*abort_flag; tile += gridDim.x) {
                 const int m0 = tile / n_tiles * 128, n0 = tile % n_tiles * BN;
-                for (int kb = 0; kb < k_iters; ++kb) {
+                for (int kb = 0; kb < k_iters; kb += C::GROUP) {
                     if (!mbar_wait(&empty[stage], phase ^ 1)) {
                         report(status, DEV_TIMEOUT);
                         *abort_flag = 1;
                         break;
                     }
-                    uint8_t *a_dst = ring + stage * C::STAGE;
-                    mbar_arrive_expect_tx(&full[stage], C::STAGE);
-                    tma_load_2d(a_dst, &tm_x, &full[stage], kb * BK, m0);
-                    tma_load_2d(a_dst + C::A_BYTES, &tm_w, &full[stage], kb * BK, n0);
+                    const int blocks = min(C::GROUP, k_iters - kb);
+                    mbar_arrive_expect_tx(&full[stage], blocks * (x_rows(M) * BK + C::B_BYTES));
+#pragma unroll
+                    for (int g = 0; g < C::GROUP; ++g)
+                        if (g < blocks) {
+                            uint8_t *a_dst = ring + stage * C::STAGE + g * C::BLOCK;
+                            tma_load_2d(a_dst, &tm_x, &full[stage], (kb + g) * BK, m0);
+                            tma_load_2d(a_dst + C::A_BYTES, &tm_w, &full[stage], (kb + g) * BK, n0);
+                        }
                     armed |= 1u << stage;
                     armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
                     if (++stage == C::STAGES) {
@@ -456,18 +470,22 @@ __global__ void __launch_bounds__(CtaCfg<BN>::THREADS, 1)
             }
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + acc * BN;
-            for (int kb = 0; kb < k_iters; ++kb) {
+            for (int kb = 0; kb < k_iters; kb += C::GROUP) {
                 if (!warp_wait(&full[stage], phase)) {
                     report(status, DEV_TIMEOUT);
                     *abort_flag = 1;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t a_addr = smem_u32(ring + stage * C::STAGE);
-                const uint64_t ad = sdesc_sw128(a_addr, 16, 1024), bd = sdesc_sw128(a_addr + C::A_BYTES, 16, 1024);
 #pragma unroll
-                for (int k = 0; k < BK / 32; ++k)  // +32 bytes per K step inside the swizzle atom
-                    if (leader) umma_f8_ss(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+                for (int g = 0; g < C::GROUP; ++g) {
+                    const uint32_t a_addr = smem_u32(ring + stage * C::STAGE + g * C::BLOCK);
+                    const uint64_t ad = sdesc_sw128(a_addr, 16, 1024), bd = sdesc_sw128(a_addr + C::A_BYTES, 16, 1024);
+                    if (leader && kb + g < k_iters)
+#pragma unroll
+                        for (int k = 0; k < BK / 32; ++k)  // +32 bytes per K step inside the swizzle atom
+                            umma_f8_ss(d_tmem, ad + 2 * k, bd + 2 * k, idesc, (kb | g | k) != 0 ? 1u : 0u);
+                }
                 issued = true;
                 if (leader) umma_commit(&empty[stage]);
                 if (++stage == C::STAGES) {
@@ -762,7 +780,7 @@ cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, co
     const int sms = current_sm_count();
     // The narrowest tiles of 64 and 128 columns that are one round of the SMs, else pairs; without the rows
     // for those (or the columns), 256 columns where that is no more work per SM than 128.  At K =
-    // 4,096: 1,024 x 1,024 is 128 tiles of 64, 10.7 us (of 128 11.2, 16 pairs 15.6); 2,048 x 1,024 128 of
+    // 4,096: 1,024 x 1,024 is 128 tiles of 64, 9.6 us (of 128 11.2, 16 pairs 15.6); 2,048 x 1,024 128 of
     // 128, 12.1 (pairs 15.9, two rounds of 64 17.5); 4,099 x 1,024 68 pairs, 16.8 (two rounds of 128 19.4);
     // 300 x 8,192 96 of 256, 16.7 (192 of 128 18.7); 300 x 16,384 384 of 128, 27.8 (192 of 256 34.0).
     auto tiles = [&](int64_t bn) { return (m + 127) / 128 * ((n + bn - 1) / bn); };
@@ -771,7 +789,7 @@ cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, co
     // the gated epilogues pair 32 gate with 32 input columns and fill a slab from 128
     const int bn = pair ? 128 : !glu && tiles(64) <= sms ? 64 : n > 128 && tiles(128) > sms && 2 * rounds(256) <= rounds(128) ? 256 : 128;
     Maps t;
-    fe_status r = make_tmap_2d(&t.x, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, m, k, k, 128, BK);
+    fe_status r = make_tmap_2d(&t.x, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, m, k, k, x_rows(static_cast<int>(m)), BK);
     if (r == FE_OK) r = make_tmap_2d(&t.w, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, n, k, k, bn, BK);
     if (r == FE_OK)
         r = bf16 ? make_tmap_2d(&t.y, y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, m, ny, ny, 32, 64)
