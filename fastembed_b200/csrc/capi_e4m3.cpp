@@ -22,7 +22,7 @@ fe_status unsupported(const char *name, const char *what) { return fail(FE_ERR_U
 fe_status check_rows(const char *name, fe_dtype dtype, int64_t rows, int32_t dim)
 {
     if (rows < 0 || dim <= 0) return bad(name, "bad shape");
-    if (rows > 0x7fffffff) return unsupported(name, "too many rows");
+    if (rows > 0x7fffffff || dim > 1 << 30) return unsupported(name, "too many rows or columns");
     if (dtype != FE_DTYPE_F32 && dtype != FE_DTYPE_BF16) return bad(name, "unknown input dtype");
     return FE_OK;
 }
@@ -42,6 +42,14 @@ fe_status check_cache(const char *name, int32_t batch, int32_t max_len, int64_t 
     if (static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_len) * (q_heads / kv_heads) + 7) / 8 + max_len / 16 + 2) >
         0x7fffffff)
         return unsupported(name, "batch x max_len too large");
+    return FE_OK;
+}
+
+// Tiles of 128 or 256 rows of a sequence's key-value head are a launch's z extent.
+fe_status check_rows_per_head(const char *name, int32_t max_len, int32_t q_heads, int32_t kv_heads)
+{
+    if (static_cast<int64_t>(max_len) * (q_heads / kv_heads) > 65535 * 128)
+        return unsupported(name, "max_len x q_heads / kv_heads too large");
     return FE_OK;
 }
 
@@ -135,6 +143,7 @@ fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int
     const char *name = "fe_attention_cache_workspace_bytes";
     if (!bytes) return bad(name, "null pointer");
     FE_TRY(check_cache(name, batch, max_len, total_tokens, q_heads, kv_heads, head_dim, 0, 0, 16));
+    FE_TRY(check_rows_per_head(name, max_len, q_heads, kv_heads));
     if (max_kv_len < 0) return bad(name, "bad shape");
     *bytes = batch == 0 || total_tokens == 0 || max_len == 0
                  ? 0
@@ -151,6 +160,7 @@ fe_status fe_attention_cache_e4m3(const void *qkv, const int32_t *cu_seqlens, in
 {
     const char *name = "fe_attention_cache_e4m3";
     FE_TRY(check_cache(name, batch, max_len, total_tokens, q_heads, kv_heads, head_dim, table_width, pages, page_size));
+    FE_TRY(check_rows_per_head(name, max_len, q_heads, kv_heads));
     if (max_kv_len < 0 || !std::isfinite(scale)) return bad(name, "bad max_kv_len or scale");
     if (batch == 0 || total_tokens == 0 || max_len == 0) return FE_OK;
     FE_TRY(check_pool(name, pages, kv_heads, page_size));

@@ -12,10 +12,11 @@
 // TMA boxes have the bf16 linear layer's geometry with half as many k-blocks: the mainloop of a
 // tile takes half as long while its epilogue costs the same, and below K = 2048 the epilogue
 // decides.  Hence eight epilogue warps in the pair kernel.
-//   linear_e4m3_pair  a cluster pair computes a 256 x 256 tile (cta_group::2); m >= 512.
-//   linear_e4m3_cta   one CTA, 128 x BN tiles; BN shrinks (256, 128, 64) until there are as
-//                     many tiles as SMs: few rows mean reading the weight, and that wants every
-//                     SM's loads in flight.
+//   linear_e4m3_pair  a cluster pair computes a 256 x 256 tile (cta_group::2); calls of more than
+//                     a round of the SMs' tiles.
+//   linear_e4m3_cta   one CTA, 128 x BN tiles; few rows mean reading the weight, and that wants
+//                     every SM's loads in flight, so BN is the smallest that is one round of them.
+// K is never split: a row's result has the same bits in whatever batch, and so kernel, it comes.
 // Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (an elected lane), then the epilogue.
 // Every mbarrier wait is bounded; on timeout the CTA records FE_ERR_DEVICE_TIMEOUT in the device
 // status word, lets its own copies and MMAs land, frees its TMEM and exits.

@@ -363,6 +363,7 @@ fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int
  * positive numbers or 0; value codes of visible tokens must not be NaN (append writes none).
  * Weights are f16 relative to the row's largest (weights times value scales): 11 bits each, and
  * 2^-32 of the largest at the least; sums are fp32.
+ * max_len * q_heads / kv_heads is at most 65,535 * 128.
  * Calls that share a workspace must not run concurrently; its contents need no initialisation. */
 fe_status fe_attention_cache_e4m3(const void *qkv, const int32_t *cu_seqlens, int32_t batch, int32_t max_len,
                                   int64_t total_tokens, int32_t q_heads, int32_t kv_heads, int32_t head_dim,

@@ -117,3 +117,18 @@ def test_front_end_refuses_host_tensors(fe_lib):
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError):
         ops.kv_cache_append_e4m3(torch.zeros(1, 8 * 64, dtype=torch.bfloat16), i, 1, i[:1], i[None], cache, 4)
+
+
+def test_attention_cache_rows_past_a_grid_are_refused(fe_lib):
+    kw = dict(batch=1, total=5, hd=128, hkv=1)
+    assert _attend(fe_lib, max_len=1 << 20, hq=9, **kw) == 4 and b"max_len" in fe_lib.fe_last_error_message()
+    size = C.c_size_t(99)
+    assert fe_lib.fe_attention_cache_workspace_bytes(1, 1 << 20, 5, 100, 9, 1, 128, C.byref(size)) == 4
+    assert fe_lib.fe_attention_cache_workspace_bytes(1, 65535, 5, 100, 128, 1, 128, C.byref(size)) == 0
+
+
+def test_row_quantisers_refuse_rows_past_their_counters(fe_lib):
+    big = (1 << 30) + 8
+    assert fe_lib.fe_quantize_rows_e4m3(buf, F32, 1, big, buf, buf, None) == 4
+    assert fe_lib.fe_add_rmsnorm_e4m3(None, F32, buf, buf, 0, 1e-6, 1, big, buf, buf, None) == 4
+    assert fe_lib.fe_quantize_rows_e4m3(None, F32, 0, 1 << 30, None, None, None) == 0
