@@ -794,3 +794,67 @@ def test_linear_rows_alone_across_kernels(cuda_dev):
               r.data_ptr(), 3001, 1032, 640, capi.EPI["bias_residual"], capi.DTYPE["f32"],
               torch.cuda.current_stream().cuda_stream)
     assert torch.equal(r, whole)
+
+
+# ------------------------------------------------------------ the ends of the ranges
+def test_nothing_to_do(cuda_dev):
+    """No rows, no sequences, no tokens: empty results, nothing launched or touched."""
+    from fastembed_b200 import ops
+    z = lambda *s: torch.zeros(*s, device=cuda_dev)
+    q, s = ops.quantize_rows_e4m3(z(0, 64))
+    assert q.shape == (0, 64) and s.shape == (0,)
+    q, s = ops.add_rmsnorm_e4m3(None, z(0, 64), z(64), 1e-6)
+    assert q.shape == (0, 64)
+    w, ws = ops.quantize_rows_e4m3(torch.randn(128, 64, device=cuda_dev))
+    assert ops.linear_e4m3(q, s, w, ws).shape == (0, 128)
+    assert ops.linear_e4m3(q, s, w, ws, epilogue="swiglu").shape == (0, 64)
+    b = Batch([0, 0], [3, 0], 16, 4, 2, 64, cuda_dev, extra_rows=3)
+    cache = b.random_cache(ops)
+    before = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    rows = b.qkv  # of no sequence
+    for qkv, max_len in ((rows[:0], 0), (rows[:0], 2), (rows, 0), (rows, 2)):
+        ops.kv_cache_append_e4m3(qkv, b.cu, max_len, b.past_lens, b.table, cache, 4)
+        out = torch.full((qkv.shape[0], 4 * 64), 2.0, dtype=torch.bfloat16, device=cuda_dev)
+        ops.attention_cache_e4m3(qkv, b.cu, max_len, b.past_lens, 3, b.table, cache, 4, out=out)
+        assert torch.all(out == 2.0)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda_dev)
+    ops.kv_cache_append_e4m3(rows, b.cu[:1], 2, none, b.table[:0], cache, 4)
+    ops.attention_cache_e4m3(rows, b.cu[:1], 2, none, 3, b.table[:0], cache, 4)
+    after = (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)
+    assert all(torch.equal(x, y) for x, y in zip(before, after))
+    ops.device_status(0)
+
+
+@pytest.mark.parametrize("hd,heads", [(64, (96, 1)), (128, (128, 1)), (128, (60, 4)), (256, (40, 1))])
+@pytest.mark.parametrize("new,past,bound", [([1, 1, 2], [40, 0, 700], None), ([3, 9], [500, 20], 1 << 20), ([40], [90], 1 << 20)])
+def test_attention_cache_wide_groups(cuda_dev, hd, heads, new, past, bound):
+    """More query heads to a key-value head than a tile loads in a round, powers of two and not."""
+    from fastembed_b200 import ops
+    b = Batch(new, past, 16, *heads, hd, cuda_dev, seed=heads[0])
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    b.max_kv = bound or b.max_kv
+    _attend(b, ops, cache)
+    _attend(b, ops, cache, False)
+
+
+def test_calls_on_two_streams_at_once(cuda_dev):
+    """The same cache read on two streams side by side, each call with its own workspace."""
+    from fastembed_b200 import ops
+    b = Batch([1, 2, 60], [3000, 40, 900], 32, 16, 8, 128, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, 16)
+    other = (b.qkv.float() * 0.25).to(torch.bfloat16)
+    run = lambda q: ops.attention_cache_e4m3(q, b.cu, b.max_new, b.past_lens, 1 << 20, b.table, cache, 16)
+    want = run(b.qkv), run(other)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (st, q) in enumerate(zip(streams, (b.qkv, other))):
+            with torch.cuda.stream(st):
+                got[i].append(run(q))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+    ops.device_status(0)
