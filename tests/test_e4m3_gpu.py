@@ -858,3 +858,36 @@ def test_calls_on_two_streams_at_once(cuda_dev):
     for outs, w in zip(got, want):
         assert all(torch.equal(o, w) for o in outs)
     ops.device_status(0)
+
+
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+@pytest.mark.parametrize("new,bound", [([3, 1], None), ([90, 40], 1 << 20)])
+def test_attention_cache_query_outliers(cuda_dev, hd, heads, new, bound):
+    """One element of each query thousands of times the others (and the keys small there): the others count
+    to 2^-16 of it, by streaming and by tiles."""
+    from fastembed_b200 import ops
+    b = Batch(new, [200, 77], 32, *heads, hd, cuda_dev)
+    x = b.qkv.view(-1, heads[0] + 2 * heads[1], hd)
+    x[:, :heads[0], 5] = 4096.0
+    x[:, heads[0]:heads[0] + heads[1], 5] *= 2.0 ** -12
+    cache = ops.kv_cache_e4m3(b.pages, 32, heads[1], hd, cuda_dev)
+    for s, p in enumerate(b.past):  # the prefix, from the same distribution
+        k = torch.randn(b.pages, heads[1], 32, hd, device=cuda_dev, generator=b.g) * 40
+        cache.k.copy_(k.to(F8))
+        cache.v.copy_(torch.randn(k.shape, device=cuda_dev, generator=b.g).mul(40).to(F8))
+    cache.k_scale.fill_(2.0 ** -9)
+    cache.v_scale.fill_(2.0 ** -6)
+    cache.k.view(torch.uint8)[..., 5] = 0
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    out = ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound or b.max_kv, b.table, cache, b.q_heads)
+    scale = hd ** -0.5
+    want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, b.past, b.table, b.q_heads, True, scale)
+    ones = torch.ones_like(b.qkv)  # sum_d |k| at its largest, as the magnitudes of a query of ones
+    dot1 = ref.attention(cache, ones, b.new, b.past, b.table, b.q_heads, True, scale)[2]
+    top = x[:sum(new), :heads[0]].double().abs().amax(-1).repeat_interleave(hd, -1).view(sum(new), -1)
+    # each element of a query is off by at most 2^-16 of its row's largest, and a logit by that times
+    # scale sum_d |k|; weights pass it on in numerator and denominator
+    extra = 2.0 * (2.0 ** -16 * top * dot1) * mag * 1.1
+    err = (out[:sum(new)].double() - want).abs()
+    assert torch.all(err <= ref.attention_bound(want, mag, dot, floor, hd) + extra)
+    ops.device_status(0)
