@@ -529,32 +529,61 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     }
 }
 
-// Sums the parts of each (token, query head) row of a sequence: a warp a row.
-template <int HD>
+// Sums the parts of each (token, query head) row of a sequence, WPR warps a row: every lane has the weight
+// of two parts (there are at most 64), each warp adds up every WPR-th.
+template <int HD, int WPR>
 __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *status)
 {
-    const int lane = threadIdx.x & 31;
+    constexpr int V = HD / 32;
+    __shared__ float rest[3][HD];  // sums of the row's warps but the first
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WPR;
     grid_dep_wait();
     grid_dep_launch();
     CacheSeq sq;
     if (!load_seq(a, blockIdx.y, sq, status)) return;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (i >= static_cast<int64_t>(sq.len) * a.q_heads) return;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + warp / WPR;
+    if (i >= static_cast<int64_t>(sq.len) * a.q_heads) return;  // whole rows
     const int64_t r = static_cast<int64_t>(sq.t0) * a.q_heads + i;
-    constexpr int V = HD / 32;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(r * a.splits + s) * 2]);
-    float sum = 0.f, acc[V];
+    float2 ml[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        ml[h] = lane + 32 * h < a.splits ? *reinterpret_cast<const float2 *>(a.part_ml + (r * a.splits + lane + 32 * h) * 2)
+                                         : make_float2(-INFINITY, 0.f);
+    const float m = warp_max(fmaxf(ml[0].x, ml[1].x));
+    float k[2], sum = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const bool none = ml[h].x == -INFINITY && ml[h].y == 0.f;  // saw nothing
+        k[h] = none ? -1.f : ml[h].x == -INFINITY ? 1.f : exp2_fast(ml[h].x - m);
+        if (!none) sum += ml[h].y * k[h];
+    }
+    sum = warp_sum(sum);
+    float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (r * a.splits + s) * 2);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
-        const float k = ml.x == -INFINITY ? 1.f : exp2_fast(ml.x - m);
-        sum += ml.y * k;
-        const float *p = a.part_o + (r * a.splits + s) * HD + lane * V;
+    const float *p = a.part_o + r * a.splits * HD + lane * V;
+#pragma unroll 4
+    for (int s = part; s < a.splits; s += WPR) {
+        const float w = __shfl_sync(0xffffffffu, s < 32 ? k[0] : k[1], s & 31);
+        float x[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += p[i] * k;
+        for (int i = 0; i < V; i += 2) {
+            const float2 f = *reinterpret_cast<const float2 *>(p + s * HD + i);
+            x[i] = f.x, x[i + 1] = f.y;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = w < 0.f ? acc[i] : fmaf(x[i], w, acc[i]);
+    }
+    if constexpr (WPR > 1) {
+        if (part > 0)
+#pragma unroll
+            for (int i = 0; i < V; ++i) rest[part - 1][lane * V + i] = acc[i];
+        __syncthreads();
+        if (part > 0) return;
+#pragma unroll
+        for (int w = 0; w < WPR - 1; ++w)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += rest[w][lane * V + i];
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     __nv_bfloat16 *dst = a.out + r * HD + lane * V;
@@ -565,8 +594,9 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
 template <int HD>
 cudaError_t launch_join(const CacheArgs &a, int *status, cudaStream_t s)
 {
-    return launch_k(attn_cache_join<HD>, dim3((static_cast<unsigned>(a.max_len) * a.q_heads + 3) / 4, a.batch), dim3(128), 0,
-                    s, a, status);
+    const unsigned rows = static_cast<unsigned>(a.max_len) * a.q_heads;
+    if (a.splits > 4) return launch_k(attn_cache_join<HD, 4>, dim3(rows, a.batch), dim3(128), 0, s, a, status);
+    return launch_k(attn_cache_join<HD, 1>, dim3((rows + 3) / 4, a.batch), dim3(128), 0, s, a, status);
 }
 
 cudaError_t launch_join(const CacheArgs &a, int head_dim, int *status, cudaStream_t s)
@@ -578,6 +608,7 @@ constexpr int kStreamRows = 32;    // rows of a key-value head up to which the s
 constexpr int kStreamCtas = 2 * kSms;            // ... and with more rows up to so many CTAs, one part each, which
 constexpr int64_t kStreamTokens = int64_t{1} << 18;  // read so many tokens together
 constexpr int kClusterParts = 8;   // portable cluster size
+constexpr int kMaxParts = 64;      // two a lane where they are joined
 constexpr int kPartTokens = 128;   // a part has a run for each of four warps
 
 // 8-row tiles of a CTA: 16 rows where the registers allow it and there are more than 8
@@ -605,28 +636,33 @@ CachePlan plan_attention_cache(int batch, int max_len, int max_kv, int q_heads, 
         const int64_t tiles = (rows + attention_cache_tile_rows(head_dim) - 1) / attention_cache_tile_rows(head_dim);
         // one CTA an SM: split until they have one each, 512 tokens or more a part
         const int64_t want = std::min<int64_t>(kSms / std::max<int64_t>(1, tiles * batch * kv_heads), 65535 / tiles);
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, 64})));
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 512, kMaxParts})));
         return p;
     }
     const int64_t resident = (head_dim == 128 && per == 16 ? 2 : 3) * kSms;  // what registers allow
     const int64_t room = std::min<int64_t>(resident / ctas, kClusterParts);
-    if (room > 1 && max_kv <= 2048 * room) {
+    if (room > 1 && max_kv <= 512 * room) {
         // As many parts as all fit at once, and those short; a power of two, since clusters of 3 or 6 leave SMs of
         // their group idle.  (Clusters that do not fit wait for room: 7 parts of 32 sequences x 8 heads
-        // took 186 us as clusters and 158 with the second launch, one sequence of 2,000 tokens 8.5 and 14.9;
-        // 16 sequences of 500, 5 new tokens, 3 parts for 2 CTAs an SM 21.8 us, 2 parts 12.8.)
+        // took 186 us as clusters and 158 with the second launch; 16 sequences of 500, 5 new tokens, 3 parts
+        // for 2 CTAs an SM 21.8 us, 2 parts 12.8.  1 x 2,000 tokens 8.7 us, with the second launch 14.9.)
         while (2 * p.splits <= std::min<int64_t>(room, max_kv / kPartTokens)) p.splits *= 2;
         p.cluster = p.splits > 1;
     }
     if (p.splits == 1) {
-        // About four rounds of the resident CTAs, since sequences differ in length, of 1,024 tokens or more
-        // (a CTA costs 2.7 us beside its reading).  32 sequences of 8,000 to 16,000 tokens, 8 heads: 2
-        // rounds 159 us, 3 152, 4 150, 6 152, 8 157; 16 of 8,000: parts of 512 tokens 67 us, of 1,024 62.
-        const int64_t want = (4 * resident + ctas - 1) / ctas;
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, max_kv / 1024, 64})));
+        // Few CTAs: one round of the resident ones, 256 tokens or more a part.  1 x 16,000 tokens: 8 heads 16.7 us (8
+        // parts in a cluster 21.5), 2 heads 12.8 (21.4), head_dim 256 and 1 head 16.5 (41.5).  Else about four
+        // rounds, since sequences differ in length, of 1,024 tokens or more (a CTA costs 2.7 us beside its
+        // reading).  32 sequences of 8,000 to 16,000 tokens, 8 heads: 2 rounds 159 us, 3 152, 4 150,
+        // 6 152, 8 157; 16 of 8,000: parts of 512 tokens 67 us, of 1,024 62.
+        const int64_t fill = resident / ctas;
+        const int64_t want = fill >= 8 ? std::min(fill, max_kv / int64_t{256})
+                                       : std::min((4 * resident + ctas - 1) / ctas, max_kv / int64_t{1024});
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, kMaxParts)));
     }
-    // a CTA that has its SM to itself takes twice the warps
-    p.wide = head_dim < 256 && ctas * p.splits <= kSms;
+    // A CTA that has its SM to itself takes twice the warps; not in clusters that fill more than half of the
+    // SMs, which would wait for eight of a group (2 x 2,000 tokens, 8 heads: 15.7 us, with four warps 10.4).
+    p.wide = head_dim < 256 && ctas * p.splits <= (p.cluster ? kSms / 2 : kSms);
     return p;
 }
 

@@ -86,7 +86,7 @@ def test_attention_cache_workspace(fe_lib):
     ask = lambda batch, max_len, total, kv, hq, hkv, hd: (
         fe_lib.fe_attention_cache_workspace_bytes(batch, max_len, total, kv, hq, hkv, hd, C.byref(size)), size.value)
     assert ask(1, 1, 1, 100, 16, 8, 128) == (0, 0)          # too short to split
-    assert ask(1, 1, 1, 16000, 16, 8, 128) == (0, 0)        # eight parts or fewer meet in a cluster
+    assert ask(1, 1, 1, 4000, 16, 8, 128) == (0, 0)         # eight parts or fewer meet in a cluster
     status, need = ask(1, 1, 1, 64000, 16, 8, 128)          # one token over a very long cache
     assert status == 0 and need >= 16 * 9 * 130 * 4
     assert ask(8, 2000, 16000, 3000, 16, 8, 128) == (0, 0)  # enough CTAs without
