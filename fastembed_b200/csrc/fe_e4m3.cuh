@@ -48,10 +48,31 @@ __device__ __forceinline__ float finite_abs(float v)
     return a <= 3.402823466e38f ? a : 0.f;
 }
 
-// v * inv, or NaN where v is not finite (the saturating conversion would make an infinity 448)
-__device__ __forceinline__ float scaled_or_nan(float v, float inv)
+// v, or NaN where v is not finite (the saturating conversion would make an infinity 448)
+__device__ __forceinline__ float finite_or_nan(float v)
 {
-    return fabsf(v) <= 3.402823466e38f ? v * inv : __int_as_float(0x7fffffff);
+    return fabsf(v) <= 3.402823466e38f ? v : __int_as_float(0x7fffffff);
+}
+
+// v / scale, with inv = 1 / scale: a product, then the quotient's remainder by one fma and what it adds by another
+// (Markstein's division).  The product alone puts quotients on a border between two codes, of which rows
+// of bf16 numbers have some (7 codes of 10,000), on either side of it.  Equal to the fp32 quotient but for
+// those within 2^-46 of halfway between two fp32 numbers, and all of a bf16 v and a bf16 maximum / 448 are equal.
+// The signs are such that -0 stays -0.  The compiler's division in its place: 26,508 x 1,024 with the norm
+// 54.6 us, so 50.
+__device__ __forceinline__ float div_by(float v, float scale, float inv)
+{
+    const float p = -v * -inv;
+    return fmaf(fmaf(p, scale, -v), -inv, p);
+}
+
+__device__ __forceinline__ void div_by2(float &a, float &b, float scale, float inv)
+{
+    const float na = -a, nb = -b;
+    float p = na, q = nb, r, s;
+    mul_f32x2(p, q, -inv, -inv);
+    fma_f32x2v(r, s, p, q, scale, scale, na, nb);
+    fma_f32x2v(a, b, r, s, -inv, -inv, p, q);
 }
 
 }  // namespace fe

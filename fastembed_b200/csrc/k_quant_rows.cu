@@ -144,14 +144,18 @@ __global__ void __launch_bounds__(BLOCK ? kRowThreads : kWarpRowThreads)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[c][j]));
     m = fmaxf(row_reduce<BLOCK, true>(m, red), kTinyAmax);
-    const float inv = kE4m3Max / m;
-    if (t == 0) scale[r] = m / kE4m3Max;
+    const float s = m / kE4m3Max, inv = 1.0f / s;
+    if (t == 0) scale[r] = s;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * T + t) * 8;
         if (col < dim) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = scaled_or_nan(v[c][j], inv);
+            for (int j = 0; j < 8; j += 2) {
+                v[c][j] = finite_or_nan(v[c][j]);
+                v[c][j + 1] = finite_or_nan(v[c][j + 1]);
+                div_by2(v[c][j], v[c][j + 1], s, inv);
+            }
             *reinterpret_cast<uint2 *>(q + r * dim + col) =
                 make_uint2(pack_e4m3x4(v[c][0], v[c][1], v[c][2], v[c][3]), pack_e4m3x4(v[c][4], v[c][5], v[c][6], v[c][7]));
         }
@@ -200,16 +204,16 @@ __global__ void __launch_bounds__(kWarpRowThreads)
         }
         m = __reduce_max_sync(0xffffffffu, m);
     }
-    const float amax = fmaxf(__uint_as_float(m << 16), kTinyAmax), inv = kE4m3Max / amax;
-    if (lane == 0) scale[r] = amax / kE4m3Max;
+    const float s = fmaxf(__uint_as_float(m << 16), kTinyAmax) / kE4m3Max, inv = 1.0f / s;
+    if (lane == 0) scale[r] = s;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int col = (c * 32 + lane) * 8;
         float2 a = unpack_bf16x2(u[c].x), b = unpack_bf16x2(u[c].y), d = unpack_bf16x2(u[c].z), e = unpack_bf16x2(u[c].w);
-        mul_f32x2(a.x, a.y, inv, inv);
-        mul_f32x2(b.x, b.y, inv, inv);
-        mul_f32x2(d.x, d.y, inv, inv);
-        mul_f32x2(e.x, e.y, inv, inv);
+        div_by2(a.x, a.y, s, inv);
+        div_by2(b.x, b.y, s, inv);
+        div_by2(d.x, d.y, s, inv);
+        div_by2(e.x, e.y, s, inv);
         if (col < dim)
             *reinterpret_cast<uint2 *>(q + r * dim + col) =
                 make_uint2(pack_e4m3x4(a.x, a.y, b.x, b.y), pack_e4m3x4(d.x, d.y, e.x, e.y));
@@ -246,10 +250,10 @@ __global__ void __launch_bounds__(kRowThreads)
     float m = 0.f;
     for (int c = threadIdx.x; c < dim; c += kRowThreads) m = fmaxf(m, finite_abs(value(c)));
     m = fmaxf(row_reduce<true, true>(m, red), kTinyAmax);
-    const float inv = kE4m3Max / m;
-    if (threadIdx.x == 0) scale[r] = m / kE4m3Max;
+    const float s = m / kE4m3Max, inv = 1.0f / s;
+    if (threadIdx.x == 0) scale[r] = s;
     for (int c = threadIdx.x; c < dim; c += kRowThreads)
-        q[r * dim + c] = static_cast<uint8_t>(cvt_e4m3x2(scaled_or_nan(value(c), inv), 0.f));
+        q[r * dim + c] = static_cast<uint8_t>(cvt_e4m3x2(div_by(finite_or_nan(value(c)), s, inv), 0.f));
 }
 
 struct RowArgs {
