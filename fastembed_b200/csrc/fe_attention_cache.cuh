@@ -14,7 +14,7 @@ struct CacheArgs {
     const float *ks, *vs;
     __nv_bfloat16 *out;
     float *part_o;  // [T * q_heads][splits][hd], splits > 1
-    float *part_ml; // [T * q_heads][splits][2]: reference exponent, sum
+    float *part_mn; // [T * q_heads][splits][4]: reference of O, of the sum, the sum, -
     int64_t total, row;
     int batch, max_len, width, pages, page_log2, q_heads, kv_heads, group, causal;
     int splits;
@@ -48,6 +48,31 @@ __device__ __forceinline__ float exp2_fast(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// A part of a row's softmax: its sum of weights times codes is 2^m O, its sum of weights 2^n l.  Each has a
+// reference of its own, since a page's value scale (any size, 0 among them) is in the first sum's weights only.
+// Without a reference (-inf) O or l is zero, or a NaN that stays.
+struct RowPart {
+    float m, n, l;
+};
+
+// What a part's O or l counts for beside the references' maximum
+__device__ __forceinline__ float part_weight(float reference, float top)
+{
+    return reference == -INFINITY ? 1.f : exp2_fast(reference - top);
+}
+
+// 1 / l (0 for a row that sees nothing) and 2^(m - n) in two factors, each of them in range
+struct RowFactor {
+    float inv, a, b;
+    __device__ __forceinline__ float operator()(float o) const { return o * inv * a * b; }
+};
+
+__device__ __forceinline__ RowFactor row_factor(float m, float n, float l)
+{
+    const float x = m == -INFINITY ? 0.f : m - n, half = truncf(0.5f * x);
+    return {l == 0.f ? 0.f : 1.0f / l, exp2_fast(half), exp2_fast(x - half)};
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)

@@ -6,10 +6,12 @@
 // head.  The scales leave the products:
 //     s_ij = (scale log2 e) sk q_i . kc_j          (base-2 logits)
 //     t_ij = s_ij + log2 sv,   P_ij = 2^(t_ij - m_i),   m_i = max_j t_ij - 15
-//     out_i = (sum_j P_ij vc_j) / (sum_j 2^(s_ij - m_i))
-// so the value scale moves into the exponent, the running maximum is that of the weights as they
+//     out_i = 2^(m_i - n_i) (sum_j P_ij vc_j) / (sum_j 2^(s_ij - n_i)),   n_i = max_j s_ij
+// so the value scale moves into the exponent, the running maximum m is that of the weights as they
 // meet the codes, and P (at most 2^15) keeps 11 bits in f16 with nothing above 2^-39 of the
-// largest weight lost, whatever the pages' scales are.  Statistics and sums are fp32.
+// largest weight lost, whatever the pages' scales are.  A page of zero values (sv = 0: t = -inf) takes part
+// in the sum of weights only, and that sum has a reference of its own, which no value scale moves.
+// Statistics and sums are fp32.
 //
 // attn_cache_stream: the form for few rows (single tokens).  A key-value head's rows are its
 // query heads' new tokens together, r = token * group + head, 8 NR of them to a CTA.  Nothing is
@@ -100,7 +102,7 @@ struct StreamCfg {
     static constexpr uint32_t STAGE = U * 2 * TILE + 16; // K, V of each tile, then sk, sv of both
     static constexpr uint32_t RING = STAGES * STAGE;     // of a warp
     static constexpr int LD = HD + 4;                    // floats per row of the joining buffer
-    static constexpr uint32_t JOIN = (WARPS * ROWS * (LD + 2) + ROWS * 2) * 4;
+    static constexpr uint32_t JOIN = (WARPS * ROWS * (LD + 4) + ROWS * 4) * 4;
     static constexpr uint32_t SMEM = WARPS * RING > JOIN ? WARPS * RING : JOIN;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
@@ -139,13 +141,6 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
     return v;
 }
 
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr)
-{
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
 // CLUSTER: the launch's parts (gridDim.z of them) are one cluster along z.
 template <int HD, int NR, int WARPS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs a, int row_tiles, int *status)
@@ -156,7 +151,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     constexpr int VC = HD >= 128 ? HD / 128 : 1;
     constexpr int VW = VB / 4;             // words of those
     constexpr int MT = HD / 16;            // m-tiles of O^T
-    // the warps' rings; at the end [WARPS][ROWS][LD], then [WARPS][ROWS][2], then [ROWS][2] floats
+    // the warps' rings; at the end [WARPS][ROWS][LD], then [WARPS][ROWS][4], then [ROWS][4] floats
     extern __shared__ __align__(16) float join[];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -233,14 +228,15 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     const int run0 = split * per, run1 = min(run0 + per, runs);
 
     float o[NR][MT][4];
-    float mx[NR][2], l[NR][2];
+    float mx[NR][2];            // the row's reference for O
+    float nx[NR][2], l[NR][2];  // the lane's own for its part of the sum
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[n][i][j] = 0.f;
-        mx[n][0] = mx[n][1] = -INFINITY;
+        mx[n][0] = mx[n][1] = nx[n][0] = nx[n][1] = -INFINITY;
         l[n][0] = l[n][1] = 0.f;
     }
 
@@ -332,14 +328,14 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                     for (int n = 0; n < NR; ++n) mma_f16(s[n][u], a0, a1, a2, a3, qf[n][j][q][0], qf[n][j][q][1]);
                 }
             }
-        // base-2 logits, masked; t = s + log2 sv (a page of zero values adds nothing: log2 -> 0)
+        // base-2 logits, masked; t = s + log2 sv (-inf for a page of zero values: it adds to the sum alone)
         float ev[2];
 #pragma unroll
-        for (int u = 0; u < C::U; ++u) ev[u] = sv[u] > 0.f ? log2f(sv[u]) : 0.f;
+        for (int u = 0; u < C::U; ++u) ev[u] = sv[u] > 0.f ? log2f(sv[u]) : -INFINITY;
         uint32_t pt[NR][C::U][2];  // P^T fragments [tile][tokens 2c.. / 2c + 8..]
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            float top[2] = {mx[n][0], mx[n][1]};
+            float top[2] = {mx[n][0], mx[n][1]}, sum_top[2] = {nx[n][0], nx[n][1]};
 #pragma unroll
             for (int u = 0; u < C::U; ++u)
 #pragma unroll
@@ -348,6 +344,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                     const bool on = sv[u] >= 0.f && tok <= lim[n][i & 1];
                     s[n][u][i] = on ? s[n][u][i] * (sk[u] * qs[n][i & 1]) : -INFINITY;
                     top[i & 1] = fmaxf(top[i & 1], s[n][u][i] + ev[u]);
+                    sum_top[i & 1] = fmaxf(sum_top[i & 1], s[n][u][i]);
                 }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -361,7 +358,6 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
                 for (int h = 0; h < 2; ++h) {
                     f[h] = mx[n][h] == -INFINITY ? 0.f : exp2_fast(mx[n][h] - top[h]);
                     mx[n][h] = top[h];
-                    l[n][h] *= f[h];
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
@@ -373,13 +369,20 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
             }
             const float ref[2] = {mx[n][0] == -INFINITY ? 0.f : mx[n][0] - kBoost,
                                   mx[n][1] == -INFINITY ? 0.f : mx[n][1] - kBoost};
+            float sum_ref[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sum_ref[h] = sum_top[h] == -INFINITY ? 0.f : sum_top[h];
+                l[n][h] *= exp2_fast(nx[n][h] - sum_ref[h]);
+                nx[n][h] = sum_top[h];
+            }
 #pragma unroll
             for (int u = 0; u < C::U; ++u) {
                 float p[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     p[i] = exp2_fast(s[n][u][i] + ev[u] - ref[i & 1]);
-                    l[n][i & 1] += exp2_fast(s[n][u][i] - ref[i & 1]);
+                    l[n][i & 1] += exp2_fast(s[n][u][i] - sum_ref[i & 1]);
                 }
                 pt[n][u][0] = transpose8x8(pack_f16x2(p[0], p[1]));
                 pt[n][u][1] = transpose8x8(pack_f16x2(p[2], p[3]));
@@ -439,20 +442,20 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     cp_async_wait<0>();
     __syncthreads();  // the rings become the joining buffer
 
-    // join the warps: each leaves its rows' m, l and O, then the CTA sums them
-    float *ml = join + WARPS * C::ROWS * C::LD, *cml = ml + WARPS * C::ROWS * 2;
+    // join the warps: each leaves its rows' references, sum and O, then the CTA adds them up
+    float4 *mn = reinterpret_cast<float4 *>(join + WARPS * C::ROWS * C::LD), *cmn = mn + WARPS * C::ROWS;
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float t = l[n][h];
+            float top = nx[n][h];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float t = l[n][h] * part_weight(nx[n][h], top);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
             const int r = 8 * n + 2 * c + h;
-            if (g == 0) {
-                ml[(warp * C::ROWS + r) * 2] = mx[n][h];
-                ml[(warp * C::ROWS + r) * 2 + 1] = t;
-            }
+            if (g == 0) mn[warp * C::ROWS + r] = make_float4(mx[n][h] - kBoost, top, t, 0.f);
             float *dst = join + (warp * C::ROWS + r) * C::LD;
 #pragma unroll
             for (int j = 0; j < VC; ++j)
@@ -466,37 +469,36 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
     for (int i = threadIdx.x; i < C::ROWS * HD / 4; i += 32 * WARPS) {
         const int r = i / (HD / 4), hd = i % (HD / 4) * 4;
         if (r0 + r >= rows) break;
-        float m = -INFINITY;
+        RowPart sum{-INFINITY, -INFINITY, 0.f};
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml[(w * C::ROWS + r) * 2]);
-        float sum = 0.f;
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 p = mn[w * C::ROWS + r];
+            sum.m = fmaxf(sum.m, p.x);
+            sum.n = fmaxf(sum.n, p.y);
+        }
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float wm = ml[(w * C::ROWS + r) * 2];
-            const float f = wm == -INFINITY ? 0.f : exp2_fast(wm - m);
-            const float wl = ml[(w * C::ROWS + r) * 2 + 1];
+            const float4 p = mn[w * C::ROWS + r];
             const float4 x = *reinterpret_cast<const float4 *>(join + (w * C::ROWS + r) * C::LD + hd);
-            if (wm != -INFINITY || wl != 0.f) {  // NaN logits leave m behind: l carries them
-                const float k = wm == -INFINITY ? 1.f : f;
-                sum += wl * k;
-                acc.x += x.x * k, acc.y += x.y * k, acc.z += x.z * k, acc.w += x.w * k;
-            }
+            const float k = part_weight(p.x, sum.m);
+            sum.l += p.z * part_weight(p.y, sum.n);
+            acc.x += x.x * k, acc.y += x.y * k, acc.z += x.z * k, acc.w += x.w * k;
         }
         if constexpr (CLUSTER) {  // this CTA's part, for the cluster to read
             *reinterpret_cast<float4 *>(join + r * C::LD + hd) = acc;  // only this thread has read it
-            if (hd == 0) *reinterpret_cast<float2 *>(cml + 2 * r) = make_float2(m, sum);
+            if (hd == 0) cmn[r] = make_float4(sum.m, sum.n, sum.l, 0.f);
             continue;
         }
         const int64_t orow = (sq.t0 + (r0 + r) / a.group) * static_cast<int64_t>(a.q_heads) + kvh * a.group + (r0 + r) % a.group;
         if (a.splits == 1) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // a row that sees nothing is zero
+            const RowFactor f = row_factor(sum.m, sum.n, sum.l);
             *reinterpret_cast<uint2 *>(a.out + orow * HD + hd) =
-                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+                make_uint2(pack_bf16x2(f(acc.x), f(acc.y)), pack_bf16x2(f(acc.z), f(acc.w)));
         } else {
             const int64_t at = orow * a.splits + split;
             *reinterpret_cast<float4 *>(a.part_o + at * HD + hd) = acc;
-            if (hd == 0) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, sum);
+            if (hd == 0) *reinterpret_cast<float4 *>(a.part_mn + at * 4) = make_float4(sum.m, sum.n, sum.l, 0.f);
         }
     }
     if constexpr (CLUSTER) {
@@ -506,23 +508,25 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
         for (int i = split + parts * threadIdx.x; i < C::ROWS * HD / 4; i += parts * 32 * WARPS) {
             const int r = i / (HD / 4), hd = i % (HD / 4) * 4;
             if (r0 + r >= rows) break;
-            float m = -INFINITY;
-            for (int k = 0; k < parts; ++k) m = fmaxf(m, ld_cluster2(map_to_rank(cml + 2 * r, k)).x);
-            float sum = 0.f;
+            RowPart sum{-INFINITY, -INFINITY, 0.f};
+            for (int k = 0; k < parts; ++k) {
+                const float4 p = ld_cluster4(map_to_rank(cmn + r, k));
+                sum.m = fmaxf(sum.m, p.x);
+                sum.n = fmaxf(sum.n, p.y);
+            }
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int k = 0; k < parts; ++k) {
-                const float2 p = ld_cluster2(map_to_rank(cml + 2 * r, k));
-                if (p.x == -INFINITY && p.y == 0.f) continue;  // saw nothing
-                const float f = p.x == -INFINITY ? 1.f : exp2_fast(p.x - m);
+                const float4 p = ld_cluster4(map_to_rank(cmn + r, k));
                 const float4 x = ld_cluster4(map_to_rank(join + r * C::LD + hd, k));
-                sum += p.y * f;
+                const float f = part_weight(p.x, sum.m);
+                sum.l += p.z * part_weight(p.y, sum.n);
                 acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
             }
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            const RowFactor f = row_factor(sum.m, sum.n, sum.l);
             const int64_t orow =
                 (sq.t0 + (r0 + r) / a.group) * static_cast<int64_t>(a.q_heads) + kvh * a.group + (r0 + r) % a.group;
             *reinterpret_cast<uint2 *>(a.out + orow * HD + hd) =
-                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+                make_uint2(pack_bf16x2(f(acc.x), f(acc.y)), pack_bf16x2(f(acc.z), f(acc.w)));
         }
         __syncthreads();
         cluster_sync();  // no CTA leaves while another reads its part
@@ -544,20 +548,23 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
     const int64_t i = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + warp / WPR;
     if (i >= static_cast<int64_t>(sq.len) * a.q_heads) return;  // whole rows
     const int64_t r = static_cast<int64_t>(sq.t0) * a.q_heads + i;
-    float2 ml[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        ml[h] = lane + 32 * h < a.splits ? *reinterpret_cast<const float2 *>(a.part_ml + (r * a.splits + lane + 32 * h) * 2)
-                                         : make_float2(-INFINITY, 0.f);
-    const float m = warp_max(fmaxf(ml[0].x, ml[1].x));
-    float k[2], sum = 0.f;
+    RowPart p2[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const bool none = ml[h].x == -INFINITY && ml[h].y == 0.f;  // saw nothing
-        k[h] = none ? -1.f : ml[h].x == -INFINITY ? 1.f : exp2_fast(ml[h].x - m);
-        if (!none) sum += ml[h].y * k[h];
+        p2[h] = {-INFINITY, -INFINITY, 0.f};
+        if (lane + 32 * h < a.splits) {
+            const float4 p = *reinterpret_cast<const float4 *>(a.part_mn + (r * a.splits + lane + 32 * h) * 4);
+            p2[h] = {p.x, p.y, p.z};
+        }
     }
-    sum = warp_sum(sum);
+    RowPart sum{warp_max(fmaxf(p2[0].m, p2[1].m)), warp_max(fmaxf(p2[0].n, p2[1].n)), 0.f};
+    float k[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        k[h] = part_weight(p2[h].m, sum.m);
+        sum.l += p2[h].l * part_weight(p2[h].n, sum.n);
+    }
+    sum.l = warp_sum(sum.l);
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
             x[i] = f.x, x[i + 1] = f.y;
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = w < 0.f ? acc[i] : fmaf(x[i], w, acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(x[i], w, acc[i]);
     }
     if constexpr (WPR > 1) {
         if (part > 0)
@@ -585,10 +592,10 @@ __global__ void __launch_bounds__(128) attn_cache_join(const CacheArgs a, int *s
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] += rest[w][lane * V + i];
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const RowFactor f = row_factor(sum.m, sum.n, sum.l);
     __nv_bfloat16 *dst = a.out + r * HD + lane * V;
 #pragma unroll
-    for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t *>(dst + i) = pack_bf16x2(f(acc[i]), f(acc[i + 1]));
 }
 
 template <int HD>
@@ -724,7 +731,7 @@ size_t attention_cache_workspace_bytes(int batch, int max_len, int64_t total, in
                                        int head_dim)
 {
     const CachePlan p = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
-    return p.workspace() ? static_cast<size_t>(total) * q_heads * p.splits * (head_dim + 2) * sizeof(float) : 0;
+    return p.workspace() ? static_cast<size_t>(total) * q_heads * p.splits * (head_dim + 4) * sizeof(float) : 0;
 }
 
 cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int batch, int max_len, int64_t total,
@@ -749,7 +756,7 @@ cudaError_t launch_attention_cache_e4m3(const void *qkv, const int32_t *cu, int 
     const CachePlan plan = plan_attention_cache(batch, max_len, max_kv, q_heads, kv_heads, head_dim);
     a.splits = plan.splits;
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = a.part_o + total * q_heads * a.splits * head_dim;
+    a.part_mn = a.part_o + total * q_heads * a.splits * head_dim;
     int *status = current_device_status_word();
     if (plan.tiles) {
         cudaError_t e = launch_attention_cache_tiles(a, head_dim, status, s, st);

@@ -1,7 +1,10 @@
 // k_attention_cache_tiles.cu — attention over the paged 8-bit key-value cache on tcgen05, for
 // prompts (many rows per key-value head).  The mathematics is that of k_attention_cache.cu:
 //     s_ij = qf_i sk(j) (q_i . kc_j),  t_ij = s_ij + log2 sv(j),  P_ij = 2^(t_ij - m_i)
-//     out_i = sum_j P_ij vc_j / sum_j P_ij / sv(j)
+//     out_i = 2^(m_i - n_i) sum_j P_ij vc_j / sum_j 2^(s_ij - n_i)
+// While the pages' value scales lie within 2^30 of the first one's, sv0, the sum of weights comes from the same
+// exponentials: 2^(s_ij - n_i) = P_ij sv0 / sv(j) with n_i = m_i - log2 sv0.  From the first page that is further
+// off (or has nothing but zeros, sv = 0) on, it has exponentials and a running reference n_i of its own.
 //
 // A unit is (sequence, key-value head, ROWS rows), the rows being the new tokens times the
 // query heads of the group, r = token * group + head, so one pass over the cache serves every
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     uint8_t *sK = sQ + NS * 2 * C::KT;          // [KS]
     uint8_t *sR = sK + KS * C::KT;              // [RS] raw V
     uint8_t *sV = sR + RS * C::KT;              // [VS] f16 V, HD / 64 boxes of 128 rows x 128 bytes
-    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, 1 / sv, (group 0) spread flag
+    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, sv0 / sv, (group 0) spread flag, (1) log2 sv0
     uint64_t *bars = reinterpret_cast<uint64_t *>(ent + kEnt * 8);
     uint64_t *k_full = bars;            // [KS]
     uint64_t *k_empty = k_full + KS;    // [KS] a commit per stream
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         const int page = 1 << a.page_log2, ppi = a.page_log2 >= 7 ? 1 : TK >> a.page_log2;  // pages per item
         const int64_t none = static_cast<int64_t>(a.pages) * a.kv_heads << a.page_log2;     // a row outside the pool
         const int32_t *tab = a.table + static_cast<int64_t>(b) * a.width;
-        float ref = 0.f;
+        float ref = 0.f, ref_sv = 1.f;
         bool have_ref = false, spread = false;
         bool ok = true;
         int kn = 0, vn = 0;
@@ -275,18 +278,20 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 const int64_t ph = row >> a.page_log2;
                 const float sv = __ldg(a.vs + ph);
                 e.x = __ldg(a.ks + ph);
-                e.y = sv > 0.f ? log2f(sv) : 0.f;  // a page of zero values adds nothing to O
-                e.z = sv > 0.f ? 1.0f / sv : 1.f;
+                if (sv > 0.f) e.y = log2f(sv);
+                e.z = sv;
             }
-            const uint32_t there = __ballot_sync(0xffffffffu, row != none);
-            if (there && !have_ref) {
-                ref = __shfl_sync(0xffffffffu, e.y, __ffs(there) - 1);
+            const uint32_t valued = __ballot_sync(0xffffffffu, e.z > 0.f);
+            if (valued && !have_ref) {
+                ref = __shfl_sync(0xffffffffu, e.y, __ffs(valued) - 1);
+                ref_sv = __shfl_sync(0xffffffffu, e.z, __ffs(valued) - 1);
                 have_ref = true;
             }
-            spread |= __any_sync(0xffffffffu, row != none && fabsf(e.y - ref) > 30.f);
+            spread |= __any_sync(0xffffffffu, row != none && !(fabsf(e.y - ref) <= 30.f));
+            if (row != none) e.z = spread ? 1.f : ref_sv / e.z;
             if (!wait(&k_empty[ks], ((n / KS) & 1) ^ 1)) return false;
             if (lane < 8) {
-                e.w = spread ? 1.f : 0.f;
+                e.w = lane == 0 ? (spread ? 1.f : 0.f) : ref;
                 ent[(n % kEnt) * 8 + lane] = e;
             }
             __syncwarp();  // the entries are written before the leader's arrival for K
@@ -479,6 +484,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         const uint32_t tO = tmem + lanes + 256 + s * HD;
         const int vis_all = __reduce_min_sync(0xffffffffu, vis);  // what every row of the warp sees
         float m_run = -INFINITY, l_run = 0.f;
+        float n_run = -INFINITY;  // the sum's reference once the scales are spread, m_run - log2 sv0 before
         bool spread = false;
         for (int k = 0; k < steps && ok; ++k) {  // 64 tokens at a time, from registers
             const int n = k >> 1, h = k & 1, c0 = 64 * h;
@@ -487,7 +493,10 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
             tc_fence_after();
             // The item's scales need no barrier of their own (226 us with one, 220 without): the producer wrote
             // them before its arrival for K, which the issuer saw before it committed S.
-            if (h == 0) spread = ent[(n % kEnt) * 8].w != 0.f;
+            if (h == 0 && !spread && ent[(n % kEnt) * 8].w != 0.f) {
+                spread = true;
+                n_run = m_run - ent[(n % kEnt) * 8 + 1].w;
+            }
             const float4 *en = ent + (n % kEnt) * 8 + (c0 >> 4);
             const int lim = vis - (j0 + n) * TK - c0;  // columns of the step that the row sees
             float alpha = 1.f;
@@ -531,13 +540,25 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                     m_run = top;
                 }
                 const float shift = m_run == -INFINITY ? 0.f : kBoost - m_run;
-                float sum = 0.f;
-                if (spread) {  // the sum's terms P / sv from their own exponentials
+                float sum = 0.f, sum_alpha = alpha;
+                if (spread) {  // the sum's terms from their own exponentials
+                    float sum_top = -INFINITY;
 #pragma unroll
                     for (int i4 = 0; i4 < 4; ++i4)
                         if (z[i4] != 0.f)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) sum += exp2_fast(fmaf(__uint_as_float(v[16 * i4 + i]), f[i4], shift));
+                            for (int i = 0; i < 16; ++i) sum_top = fmaxf(sum_top, __uint_as_float(v[16 * i4 + i]) * f[i4]);
+                    sum_alpha = 1.f;
+                    if (sum_top > n_run + kLazy) {
+                        sum_alpha = exp2_fast(n_run - sum_top);
+                        n_run = sum_top;
+                    }
+                    const float sum_shift = n_run == -INFINITY ? 0.f : kBoost - n_run;
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4)
+                        if (z[i4] != 0.f)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum += exp2_fast(fmaf(__uint_as_float(v[16 * i4 + i]), f[i4], sum_shift));
                 }
                 uint32_t pk[32];
 #pragma unroll
@@ -558,7 +579,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 }
                 __syncwarp();
                 tmem_st_x32(tS, pk);
-                l_run = fmaf(l_run, alpha, sum);
+                l_run = fmaf(l_run, sum_alpha, sum);
                 tmem_wait_st();
             }
             // O *= alpha after the previous step's PV and before this one's
@@ -583,10 +604,10 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         if (ok && steps > 0) ok = wait(&pv_done[slot_of(s, steps - 1)], phase_of(steps - 1));
         tc_fence_after();
         if (ok && warp_live) {
-            const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // a row that sees nothing is zero
+            if (!spread && items > 0) n_run = m_run - ent[((items - 1) % kEnt) * 8 + 1].w;
             if (a.splits > 1) {
                 const int64_t at = ((static_cast<int64_t>(sq.t0) + token) * a.q_heads + head) * a.splits + split;
-                if (live) *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m_run, l_run);
+                if (live) *reinterpret_cast<float4 *>(a.part_mn + at * 4) = make_float4(m_run - kBoost, n_run - kBoost, l_run, 0.f);
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     uint32_t v[32];
@@ -610,6 +631,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 // Rows leave through this warp's share of Q's shared memory (every S that reads it is
                 // done), so that whole rows are stored side by side: a lane a row would be 32 lines
                 // an instruction.  16-byte chunks are permuted by the row against bank conflicts.
+                const RowFactor f = row_factor(m_run, n_run, l_run);
                 uint8_t *rowbuf = sQ + (s * 2 * C::KT) + q * (32 * HD * 2);
                 constexpr int CH = HD / 8;  // 16-byte chunks of a row
 #pragma unroll 1
@@ -622,7 +644,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                         uint32_t o[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            o[j] = pack_bf16x2(__uint_as_float(v[8 * i + 2 * j]) * inv, __uint_as_float(v[8 * i + 2 * j + 1]) * inv);
+                            o[j] = pack_bf16x2(f(__uint_as_float(v[8 * i + 2 * j])), f(__uint_as_float(v[8 * i + 2 * j + 1])));
                         *reinterpret_cast<uint4 *>(rowbuf + lane * (HD * 2) + (((c / 8 + i) ^ (lane & 7)) << 4)) =
                             make_uint4(o[0], o[1], o[2], o[3]);
                     }

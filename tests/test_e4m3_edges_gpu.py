@@ -127,3 +127,123 @@ def test_norm_of_a_row_whose_sum_of_squares_overflows(cuda_dev):
         q, s = ops.add_rmsnorm_e4m3(None, h, w, 1e-6)
         assert torch.all(q[1].float() == 0) and float(s[1]) == float(torch.tensor(2.0 ** -110) / torch.tensor(448.0))
         assert torch.all(q[0].float() == 448) and torch.all(q[2].float() == 448)
+
+
+# ------------------------------------------------------------ value scales of pages
+def _strict(b, cache, want, mag, dot, causal, scale):
+    """How far attention may be off when nothing is granted for pages of zero values or for the size of the
+    scales.  As ref.attention_bound, with these changes: a page whose value scale is 0 adds nothing to the
+    row's largest weight as it meets the codes; the exponents that carry a scale (logit + log2 sv, minus
+    the reference, plus the reference's difference from the sum's own) are numbers of at most E = |log2 sv|
+    + 3 |logit| + 20 in base 2, and eight roundings of half a step each on them pass on ln 2 * 8 * 2^-24 E;
+    results below 2^-126 keep bf16's absolute step of 2^-133, half of it and half of fp32's 2^-149 thrice."""
+    out = torch.zeros_like(want)
+    q = b.qkv.view(b.qkv.shape[0], -1, b.hd)[:, :b.q_heads].double()
+    group, t0, floor = b.q_heads // b.kv_heads, 0, torch.zeros_like(want).view(-1, b.q_heads, b.hd)
+    e_max = torch.where(cache.v_scale > 0, cache.v_scale.double().log2().abs(), 0.0).max()
+    for s, (n, p) in enumerate(zip(b.new, b.past)):
+        at = b.table[s, : -(-(n + p) // b.page)].long()
+        k = ref.values(cache.k.view(torch.uint8)[at].view(F8), cache.k_scale[at]).transpose(0, 1).reshape(b.kv_heads, -1, b.hd)
+        k = k[:, :n + p].repeat_interleave(group, 0)
+        sv = cache.v_scale[at].double().t().repeat_interleave(b.page, 1)[:, :n + p].repeat_interleave(group, 0)
+        codes = cache.v.view(torch.uint8)[at].view(F8).float().double().abs().transpose(0, 1).reshape(b.kv_heads, -1, b.hd)
+        codes = codes[:, :n + p].repeat_interleave(group, 0)
+        keep = torch.ones(n, n + p, dtype=torch.bool, device=k.device)
+        if causal:
+            keep = keep.tril(p)
+        logits = (q[t0:t0 + n].transpose(0, 1) @ k.transpose(1, 2) * scale).masked_fill(~keep, -math.inf)
+        w = torch.softmax(logits, -1) * sv[:, None]
+        codes = torch.where(sv[..., None] > 0, codes, 0.0)
+        floor[t0:t0 + n] = (w.amax(-1, keepdim=True) * (keep.double() @ codes)).transpose(0, 1)
+        t0 += n
+    ds = (b.hd + 8) * 2.0 ** -23 * dot + math.log(2) * 8 * 2.0 ** -24 * (e_max + 3 * 1.45 * dot + 20)
+    rel = 2.0 ** -11 + 2.0 ** -19 + 2.0 * ds
+    return 2.0 ** -8 * want.abs() + rel * mag * 1.01 + 2.0 ** -32 * floor.reshape(want.shape) + 2.0 ** -133
+
+
+FORMS = [([1, 1], None), ([1, 1], 1 << 20), ([5, 2], None), ([5, 2], 1 << 20), ([80, 3], None), ([300, 90], 1 << 20)]
+
+
+def _check(b, ops, cache, bound=None, causal=True, scale=None):
+    scale = b.hd ** -0.5 if scale is None else scale
+    out = ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound or b.max_kv, b.table, cache, b.q_heads, causal, scale)
+    want, mag, dot, _ = ref.attention(cache, b.qkv, b.new, b.past, b.table, b.q_heads, causal, scale)
+    err, most = (out.double() - want).abs(), _strict(b, cache, want, mag, dot, causal, scale)
+    assert torch.all(err <= most), (float((err / most).max()), float(out.double().abs().max()), float(want.abs().max()))
+    ops.device_status(0)
+    return out
+
+
+def _zero_pages(b, cache, seq, ordinals):
+    for o in ordinals:
+        at = int(b.table[seq, o])
+        cache.v_scale[at] = 0
+        cache.v.view(torch.uint8)[at] = 0
+
+
+@pytest.mark.parametrize("new,bound", FORMS)
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+def test_zero_value_pages_leave_the_others_their_weights(cuda_dev, new, bound, hd, heads):
+    """A page of zero values beside pages of small ones (2^-40, 2^-100) and of ordinary ones, at equal logits and
+    with the zero page's tokens far ahead: its weight counts in the sum and takes nothing from the others'."""
+    from fastembed_b200 import ops
+    b = Batch(new, [500, 333], 16, *heads, hd, cuda_dev, seed=hd)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    keys = cache.k.view(torch.uint8).clone()
+    for zero in ([0], [3, 4, 9], [8, 12, 13, 14, 15, 16, 17, 18, 19, 20]):
+        for exponent in (-40, -100, -9):
+            cache.k.view(torch.uint8).copy_(keys)
+            cache.v.copy_(torch.where(cache.v.float().abs() < 2.0, 2.0, cache.v.float()).to(F8))
+            cache.v_scale.fill_(2.0 ** exponent)
+            for s in range(2):
+                _zero_pages(b, cache, s, zero)
+            _check(b, ops, cache, bound, scale=0.0)  # equal logits
+            _check(b, ops, cache, bound)
+            # the first zero page's keys along the query of token 0: some 25 to 35 in base 2 above the rest
+            q0 = b.qkv.view(b.qkv.shape[0], -1, hd)[0, : b.q_heads].float()
+            at = int(b.table[0, zero[0]])
+            for h in range(b.kv_heads):
+                unit = q0[h * (b.q_heads // b.kv_heads)]
+                cache.k[at, h] = (unit / unit.abs().max() * 400).to(F8)
+            cache.k_scale[at] = 2.0 ** -6
+            _check(b, ops, cache, bound)
+
+
+@pytest.mark.parametrize("new,bound", FORMS)
+def test_only_zero_value_pages(cuda_dev, new, bound):
+    """Nothing but pages of zero values: zeros, causal and not.  Then one page of ordinary values at the end."""
+    from fastembed_b200 import ops
+    b = Batch(new, [300, 150], 32, 4, 2, 128, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    scales, codes = cache.v_scale.clone(), cache.v.view(torch.uint8).clone()
+    cache.v_scale.zero_()
+    cache.v.view(torch.uint8).zero_()
+    for causal in (True, False):
+        assert torch.all(_check(b, ops, cache, bound, causal) == 0)
+    at = int(b.table[0, 300 // 32])
+    cache.v_scale[at] = scales[at]
+    cache.v.view(torch.uint8)[at] = codes[at]
+    _check(b, ops, cache, bound)
+
+
+@pytest.mark.parametrize("new,bound", FORMS)
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+def test_value_scales_of_any_size(cuda_dev, new, bound, hd, heads):
+    """Scales from 2^-130 to 2^117, one size in all pages and sizes far apart in either order, at equal logits too: neither
+    the sum nor a row's weights overflow or vanish."""
+    from fastembed_b200 import ops
+    b = Batch(new, [500, 333], 16, *heads, hd, cuda_dev, seed=hd + 1)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    for exps in ([-113], [-122], [-130], [117], [-80, 100], [100, -80], [-126, 0, 0, 110], [3, 2, 1, 0, -1, -2, -50, -120]):
+        e = torch.zeros(b.pages, device=cuda_dev, dtype=torch.float64)
+        for s in range(2):
+            at = b.table[s].long()
+            count = -(-(b.new[s] + b.past[s]) // 16)
+            e[at[:count]] = torch.tensor(exps, device=cuda_dev, dtype=torch.float64).repeat(count)[:count]
+        factor = 1.37 if len(exps) % 2 == 0 else 1.0  # not only powers of two
+        cache.v_scale.copy_((2.0 ** e * factor).float()[:, None].expand(-1, b.kv_heads))
+        _check(b, ops, cache, bound, scale=0.0)
+        _check(b, ops, cache, bound)
