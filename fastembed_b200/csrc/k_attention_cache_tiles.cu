@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     uint8_t *sK = sQ + NS * 2 * C::KT;          // [KS]
     uint8_t *sR = sK + KS * C::KT;              // [RS] raw V
     uint8_t *sV = sR + RS * C::KT;              // [VS] f16 V, HD / 64 boxes of 128 rows x 128 bytes
-    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, sv0 / sv, (group 0) spread flag, (1) log2 sv0
+    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, sv0 / sv, (group 0) spread flag, (1) log2 sv0, (2) first token that is there
     uint64_t *bars = reinterpret_cast<uint64_t *>(ent + kEnt * 8);
     uint64_t *k_full = bars;            // [KS]
     uint64_t *k_empty = k_full + KS;    // [KS] a commit per stream
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         const int64_t none = static_cast<int64_t>(a.pages) * a.kv_heads << a.page_log2;     // a row outside the pool
         const int32_t *tab = a.table + static_cast<int64_t>(b) * a.width;
         float ref = 0.f, ref_sv = 1.f;
+        int first_there = 0x7fffffff;  // of this CTA's items so far
         bool have_ref = false, spread = false;
         bool ok = true;
         int kn = 0, vn = 0;
@@ -281,6 +282,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                 if (sv > 0.f) e.y = log2f(sv);
                 e.z = sv;
             }
+            const uint32_t there = __ballot_sync(0xffffffffu, row != none);
+            if (there) first_there = min(first_there, (j0 + n) * TK + 16 * (__ffs(there) - 1));
             const uint32_t valued = __ballot_sync(0xffffffffu, e.z > 0.f);
             if (valued && !have_ref) {
                 ref = __shfl_sync(0xffffffffu, e.y, __ffs(valued) - 1);
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
             if (row != none) e.z = spread ? 1.f : ref_sv / e.z;
             if (!wait(&k_empty[ks], ((n / KS) & 1) ^ 1)) return false;
             if (lane < 8) {
-                e.w = lane == 0 ? (spread ? 1.f : 0.f) : ref;
+                e.w = lane == 0 ? (spread ? 1.f : 0.f) : lane == 1 ? ref : __int_as_float(first_there);
                 ent[(n % kEnt) * 8 + lane] = e;
             }
             __syncwarp();  // the entries are written before the leader's arrival for K
@@ -604,7 +607,15 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
         if (ok && steps > 0) ok = wait(&pv_done[slot_of(s, steps - 1)], phase_of(steps - 1));
         tc_fence_after();
         if (ok && warp_live) {
-            if (!spread && items > 0) n_run = m_run - ent[((items - 1) % kEnt) * 8 + 1].w;
+            // A row that sees no token of this part (its pages are out of the pool) has seen zeros, with a
+            // non-finite query NaN: it ends as it began.
+            bool sees = false;
+            if (items > 0) {
+                const float4 *last = ent + ((items - 1) % kEnt) * 8;
+                sees = vis > __float_as_int(last[2].w);
+                if (!spread) n_run = m_run - last[1].w;
+            }
+            if (!sees) m_run = n_run = -INFINITY, l_run = 0.f;
             if (a.splits > 1) {
                 const int64_t at = ((static_cast<int64_t>(sq.t0) + token) * a.q_heads + head) * a.splits + split;
                 if (live) *reinterpret_cast<float4 *>(a.part_mn + at * 4) = make_float4(m_run - kBoost, n_run - kBoost, l_run, 0.f);
@@ -614,10 +625,9 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                     if (items > 0) {
                         tmem_ld_x32(tO + c, v);
                         tmem_wait_ld_regs(v);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0;
                     }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = sees ? v[i] : 0;
                     if (live) {
                         float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * HD + c);
 #pragma unroll
@@ -639,6 +649,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
                     uint32_t v[32];
                     tmem_ld_x32(tO + c, v);
                     tmem_wait_ld_regs(v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = sees ? v[i] : 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t o[4];

@@ -247,3 +247,61 @@ def test_value_scales_of_any_size(cuda_dev, new, bound, hd, heads):
         cache.v_scale.copy_((2.0 ** e * factor).float()[:, None].expand(-1, b.kv_heads))
         _check(b, ops, cache, bound, scale=0.0)
         _check(b, ops, cache, bound)
+
+
+# ------------------------------------------------------------ pages that are not there
+@pytest.mark.parametrize("new,bound", [([3, 2], None), ([3, 2], 1 << 20), ([60, 40], None), ([90, 200], 1 << 20)])
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+def test_non_finite_queries_over_absent_pages(cuda_dev, new, bound, hd, heads):
+    """A query with a NaN or an infinity that sees no token (its pages are all out of the pool) is zero like any other;
+    one that sees some page is NaN; finite rows see what is there."""
+    from fastembed_b200 import ops
+    from fastembed_b200.capi import FeError
+    b = Batch(new, [200, 300], 32, *heads, hd, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    q = b.qkv.view(-1, heads[0] + 2 * heads[1], hd)
+    T, a = sum(new), new[0]
+    run = lambda t: ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound or b.max_kv, t, cache,
+                                             heads[0]).view(T, heads[0], hd)
+    gone, part = b.table.clone(), b.table.clone()
+    gone[0] = -5
+    part[0, ::2] = b.pages
+    finite = {"gone": run(gone).clone(), "part": run(part).clone()}
+    with pytest.raises(FeError):
+        ops.device_status(0)
+    bad = torch.zeros(T, heads[0], dtype=torch.bool, device=cuda_dev)
+    for t, h, x in ((0, 0, math.nan), (1, 2, math.inf), (2, 1, -math.inf), (a, 0, math.nan), (a + 1, 2, math.inf)):
+        q[t, h, 3] = x
+        bad[t, h] = True
+    got = run(gone).clone()
+    assert torch.all(got[:a] == 0)
+    assert torch.isnan(got[a:][bad[a:]]).all() and torch.equal(got[a:][~bad[a:]], finite["gone"][a:][~bad[a:]])
+    got = run(part).clone()
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], finite["part"][~bad])
+    with pytest.raises(FeError):
+        ops.device_status(0)
+    ops.device_status(0)
+
+
+def test_finite_queries_over_some_absent_pages(cuda_dev):
+    """What is left of a sequence when pages are missing: the softmax over the tokens of the others."""
+    from fastembed_b200 import ops
+    from fastembed_b200.capi import FeError
+    for new, bound in (([1, 1], 1 << 20), ([4, 2], 400), ([70, 40], 400), ([130, 40], 1 << 20)):
+        b = Batch(new, [256, 128], 16, 4, 2, 128, cuda_dev, seed=3)
+        cache = b.random_cache(ops)
+        ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+        table = b.table.clone()
+        gone = [1, 2, 6]
+        for o in gone:
+            table[:, o] = -1
+        out = ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound, table, cache, 4)
+        with pytest.raises(FeError):
+            ops.device_status(0)
+        # the same tokens without those pages: positions move up by their 48 tokens
+        left = [o for o in range(b.table.shape[1]) if o not in gone]
+        short = b.table[:, left].contiguous()
+        past = [p - 16 * len(gone) for p in b.past]
+        want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, past, short, 4, True, 128 ** -0.5)
+        assert torch.all((out.double() - want).abs() <= ref.attention_bound(want, mag, dot, floor, 128))
