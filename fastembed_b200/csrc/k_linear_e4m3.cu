@@ -86,7 +86,7 @@ __device__ __forceinline__ bool given_up(const volatile int *flag) { return __an
 struct EpiArgs {
     const float *sx;        // [M]
     const float *sw;        // [N]
-    const float *bias;      // [N] or null
+    const float *bias;      // [N]; null for the epilogues without one
     int epi;
 };
 
@@ -233,7 +233,7 @@ __device__ __forceinline__ void drain_glu(uint32_t t_row, int store_row, int n0,
         tmem_wait_ld_regs(g);
         tmem_wait_ld_regs(u);
         float a[32], b[32];
-        scale_bias(a, g, sx, sl.cols + c, sl.cols + COLS + c);  // the biases are 0
+        scale_bias(a, g, sx, sl.cols + c, sl.cols + COLS + c);  // no bias: zeros
         scale_bias(b, u, sx, sl.cols + c + 32, sl.cols + COLS + c + 32);
         if (c + 64 < COLS) {
             tmem_ld_x32(t_row + c + 64, g);
@@ -323,7 +323,7 @@ __device__ __forceinline__ bool finish_tile(uint64_t *acc_full, uint32_t parity,
 {
     const float sx = row < M ? __ldg(ea.sx + row) : 0.f;  // these loads overlap the wait for the accumulator
     const bool any = store_row < M && n0 < N;             // else nothing to store
-    if (any) stage_cols<COLS>(sl.cols, ea.sw, ea.epi == E_NONE ? nullptr : ea.bias, n0, N, lane);
+    if (any) stage_cols<COLS>(sl.cols, ea.sw, ea.bias, n0, N, lane);
     if constexpr (!OUT_BF16)
         if (ea.epi == E_RESID && any) start_residual<COLS>(tm_r, sl, n0, store_row, lane);
     if (!warp_wait(acc_full, parity)) return false;
@@ -810,7 +810,7 @@ cudaError_t launch_linear_e4m3(const void *x, const float *sx, const void *w, co
         *st = r;
         return cudaSuccess;
     }
-    const EpiArgs ea{sx, sw, bias, epilogue};
+    const EpiArgs ea{sx, sw, epilogue == E_NONE || glu ? nullptr : bias, epilogue};
     const int M = static_cast<int>(m), N = static_cast<int>(n), K = static_cast<int>(k);
     if (pair) return bf16 ? launch_pair<true>(t, M, N, K, ea, s) : launch_pair<false>(t, M, N, K, ea, s);
     if (bn == 256) return bf16 ? launch_cta<256, true>(t, M, N, K, ea, s) : launch_cta<256, false>(t, M, N, K, ea, s);

@@ -318,9 +318,9 @@ fe_status fe_quantize_rows_e4m3(const void *x, fe_dtype x_dtype, int64_t rows, i
 fe_status fe_add_rmsnorm_e4m3(const void *y, fe_dtype y_dtype, float *h32, const float *w, int32_t one_plus, float eps,
                               int64_t rows, int32_t dim, void *q, float *scale, fe_stream_t stream);
 /* y[m,n] = epilogue(x_scale[i] * w_scale[j] * (x[m,k] . w[n,k]^T)) over e4m3 codes, one scale
- * per row of x and of w, FP32 accumulation; the epilogues of fe_linear_bf16, gated ones included.
- * y is bf16 or fp32; activations and gates write bf16, the residual form fp32 (y may be the
- * residual itself).  k % 16 == 0, n % 8 == 0; 16-byte aligned pointers (x_scale: 4). */
+ * per row of x and of w, FP32 accumulation; the epilogues of fe_linear_bf16, gated ones included
+ * (a bias or residual that the epilogue has no place for is not read).  y is bf16 or fp32;
+ * activations and gates write bf16, the residual form fp32 (y may be the residual itself).  k % 16 == 0, n % 8 == 0; 16-byte aligned pointers (x_scale: 4). */
 fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, const float *w_scale, const float *bias,
                          const float *residual, void *y, int64_t m, int64_t n, int64_t k, fe_epilogue epilogue,
                          fe_dtype y_dtype, fe_stream_t stream);

@@ -305,3 +305,19 @@ def test_finite_queries_over_some_absent_pages(cuda_dev):
         past = [p - 16 * len(gone) for p in b.past]
         want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, past, short, 4, True, 128 ** -0.5)
         assert torch.all((out.double() - want).abs() <= ref.attention_bound(want, mag, dot, floor, 128))
+
+
+# ------------------------------------------------------------ gated linear layers have no bias
+@pytest.mark.parametrize("m,n,k", [(3, 256, 64), (130, 512, 256), (700, 1024, 256), (2000, 2304, 128)])
+@pytest.mark.parametrize("epi", ["swiglu", "geglu"])
+def test_gated_linear_takes_no_bias(cuda_dev, m, n, k, epi):
+    """The gated epilogues and "none" are without a bias, as in the bf16 linear layer: one that is passed all the same is
+    not read."""
+    from fastembed_b200 import ops
+    g = torch.Generator(device=cuda_dev).manual_seed(m)
+    x, xs = ops.quantize_rows_e4m3(torch.randn(m, k, device=cuda_dev, generator=g))
+    w, ws = ops.quantize_rows_e4m3(torch.randn(n, k, device=cuda_dev, generator=g))
+    bias = torch.randn(n, device=cuda_dev, generator=g)
+    for e in (epi, "none"):
+        assert torch.equal(ops.linear_e4m3(x, xs, w, ws, bias, None, e), ops.linear_e4m3(x, xs, w, ws, None, None, e))
+    ops.device_status(0)
