@@ -23,7 +23,7 @@ struct CacheArgs {
 
 constexpr int kMaxCacheTokens = 1 << 30;  // of a sequence: token indexes fit 32 bits with room
 
-// One sequence of the batch: false (and a report) when its offsets do not describe it.
+// One sequence of the batch: false when it is empty, and (with a report) when its offsets do not describe it.
 struct CacheSeq {
     int t0, len, past, kv;  // first row, new tokens, tokens before them, tokens in the cache
 };
@@ -33,11 +33,11 @@ __device__ __forceinline__ bool load_seq(const CacheArgs &a, int b, CacheSeq &s,
     s.t0 = a.cu[b];
     const int t1 = a.cu[b + 1];
     s.past = a.past[b];
-    s.len = t1 - s.t0;
-    if (s.len <= 0) return false;
-    const int64_t kv = static_cast<int64_t>(s.past) + s.len;
-    const bool ok = s.t0 >= 0 && t1 <= a.total && s.len <= a.max_len && s.past >= 0 && kv <= kMaxCacheTokens &&
+    if (t1 == s.t0) return false;
+    const int64_t len = static_cast<int64_t>(t1) - s.t0, kv = s.past + len;
+    const bool ok = s.t0 >= 0 && len > 0 && t1 <= a.total && len <= a.max_len && s.past >= 0 && kv <= kMaxCacheTokens &&
                     kv <= (static_cast<int64_t>(a.width) << a.page_log2);
+    s.len = static_cast<int>(len);
     s.kv = static_cast<int>(kv);
     if (!ok && threadIdx.x == 0) report(status, DEV_BAD_INPUT);
     return ok;

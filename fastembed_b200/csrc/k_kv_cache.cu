@@ -109,9 +109,9 @@ __global__ void __launch_bounds__(THREADS) kv_append(const AppendArgs a, int rea
     grid_dep_wait();
     grid_dep_launch();
     const int t0 = a.cu[b], t1 = a.cu[b + 1], past = a.past[b];
-    if (t1 <= t0) return;
-    const int64_t end = static_cast<int64_t>(past) + t1 - t0;
-    if (t0 < 0 || t1 > a.total || t1 - t0 > a.max_len || past < 0 || end > kMaxCacheTokens ||
+    if (t1 == t0) return;
+    const int64_t len = static_cast<int64_t>(t1) - t0, end = past + len;
+    if (t0 < 0 || len < 0 || t1 > a.total || len > a.max_len || past < 0 || end > kMaxCacheTokens ||
         end > static_cast<int64_t>(a.width) * a.page) {  // offsets that do not describe the batch: nothing is touched
         if (threadIdx.x == 0) report(status, DEV_BAD_INPUT);
         return;

@@ -320,7 +320,8 @@ fe_status fe_add_rmsnorm_e4m3(const void *y, fe_dtype y_dtype, float *h32, const
 /* y[m,n] = epilogue(x_scale[i] * w_scale[j] * (x[m,k] . w[n,k]^T)) over e4m3 codes, one scale
  * per row of x and of w, FP32 accumulation; the epilogues of fe_linear_bf16, gated ones included
  * (a bias or residual that the epilogue has no place for is not read).  y is bf16 or fp32;
- * activations and gates write bf16, the residual form fp32 (y may be the residual itself).  k % 16 == 0, n % 8 == 0; 16-byte aligned pointers (x_scale: 4). */
+ * activations and gates write bf16, the residual form fp32 (y may be the residual itself).
+ * k % 16 == 0, n % 8 == 0; 16-byte aligned pointers (x_scale: 4). */
 fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, const float *w_scale, const float *bias,
                          const float *residual, void *y, int64_t m, int64_t n, int64_t k, fe_epilogue epilogue,
                          fe_dtype y_dtype, fe_stream_t stream);
@@ -333,9 +334,10 @@ fe_status fe_linear_e4m3(const void *x, const float *x_scale, const void *w, con
  * [total_tokens, (q_heads + 2 kv_heads) * head_dim], rows cu_seqlens[b] .. cu_seqlens[b+1] the
  * new tokens of sequence b (at most max_len), at positions past_lens[b] and up.  head_dim 64,
  * 128 or 256.  cu_seqlens, past_lens and page_table are read on the device: a sequence whose
- * offsets do not fit (rows past total_tokens, more than max_len new tokens, more than
- * table_width pages or 2^30 tokens in all, a negative past) is left out, and so are the tokens of a page id outside [0, pages); either
- * sets FE_ERR_INVALID_ARGUMENT in the device status word. */
+ * offsets do not fit (an end before its start, rows past total_tokens, more than max_len new
+ * tokens, more than table_width pages or 2^30 tokens in all, a negative past) is left out, and so
+ * are the tokens of a page id outside [0, pages); either sets FE_ERR_INVALID_ARGUMENT in the
+ * device status word.  A sequence without new tokens is neither read nor checked. */
 
 /* Writes the new tokens' keys and values into their pages.  The scale of a (page, head) is the
  * smallest power of two s >= 2^-80 with max |v| <= 448 s over the finite values written to the

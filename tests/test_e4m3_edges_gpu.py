@@ -321,3 +321,38 @@ def test_gated_linear_takes_no_bias(cuda_dev, m, n, k, epi):
     for e in (epi, "none"):
         assert torch.equal(ops.linear_e4m3(x, xs, w, ws, bias, None, e), ops.linear_e4m3(x, xs, w, ws, None, None, e))
     ops.device_status(0)
+
+
+# ------------------------------------------------------------ offsets that run backwards
+@pytest.mark.parametrize("new,bound", [([4, 3, 2], 300), ([90, 40, 20], 300), ([90, 40, 20], 1 << 20)])
+def test_offsets_that_run_backwards_are_reported(cuda_dev, new, bound):
+    """A sequence whose end lies before its start does not fit: left out by both calls, and reported.  (Equal offsets are an
+    empty sequence, which is nothing to report.)"""
+    from fastembed_b200 import ops
+    from fastembed_b200.capi import FeError
+    b = Batch(new, [40, 33, 50], 32, 8, 2, 128, cuda_dev)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, 8)
+    T = sum(new)
+    run = lambda cu, past: ops.attention_cache_e4m3(b.qkv, cu, b.max_new, past, bound, b.table, cache, 8,
+                                                    out=torch.full((T, 8 * 128), 9.0, dtype=torch.bfloat16, device=cuda_dev))
+    want = run(b.cu, b.past_lens)
+    ops.device_status(0)
+    state = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_dev)
+    a = new[0]
+    for back in ([0, a, a - 2, a - 2], [0, a, -2147483647, -2147483647]):
+        got = run(i32(back), b.past_lens)
+        with pytest.raises(FeError):
+            ops.device_status(0)
+        assert torch.equal(got[:a], want[:a]) and torch.all(got[a:] == 9.0)
+        b.qkv[a:].neg_()
+        ops.kv_cache_append_e4m3(b.qkv, i32(back), b.max_new, b.past_lens, b.table, cache, 8)
+        b.qkv[a:].neg_()
+        with pytest.raises(FeError):
+            ops.device_status(0)
+        for was, now in zip(state, (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)):
+            assert torch.equal(was, now)
+    got = run(i32([0, a, a, a]), i32([40, -1, 50]))  # empty ones, whatever else stands there
+    assert torch.equal(got[:a], want[:a]) and torch.all(got[a:] == 9.0)
+    ops.device_status(0)
