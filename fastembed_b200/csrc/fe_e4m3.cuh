@@ -56,7 +56,7 @@ __device__ __forceinline__ float finite_or_nan(float v)
 
 // v / scale, with inv = 1 / scale: a product, then the quotient's remainder by one fma and what it adds by another
 // (Markstein's division).  The product alone puts quotients on a border between two codes, of which rows
-// of bf16 numbers have some (7 codes of 10,000), on either side of it.  Equal to the fp32 quotient but for
+// of bf16 numbers have some (3 codes of 10,000), on either side of it.  Equal to the fp32 quotient but for
 // those within 2^-46 of halfway between two fp32 numbers, and all of a bf16 v and a bf16 maximum / 448 are equal.
 // The signs are such that -0 stays -0.  The compiler's division in its place: 26,508 x 1,024 with the norm
 // 54.6 us, so 50.

@@ -10,13 +10,14 @@
 // query heads of the group, r = token * group + head, so one pass over the cache serves every
 // query head that shares it.  A unit is one CTA: NS streams of 128 rows (two for head_dim 64
 // and 128) over the same 128-token items, each with its own S, O and softmax warpgroup.  Units go
-// out longest first (a causal prompt's last tile sees the most tokens); a unit's items may be
-// split over CTAs.
+// out by tile, the last tile of every sequence first: longest first where the prompts are about as long as each
+// other (a causal prompt's last tile sees the most tokens).  Beside a prompt, a single token over a long cache
+// has its only tile at the end of that order.  A unit's items may be split over CTAs.
 //
 //   Steps of 64 tokens: a stream has two 64-column S slots in TMEM, S of a step goes into the
 //     slot that the step before the last has left, and so S(k + 1) and PV(k - 1) run under the
 //     softmax of step k.  (One 128-column slot per stream, where S had to wait for the previous
-//     PV, took 250 us where this took 224: 8 prompts of 2,000 tokens after 1,000, 16 heads to 8, now 219.)
+//     PV, took 250 us where this took 224: 8 prompts of 2,000 tokens after 1,000, 16 heads to 8, now 215.)
 //   K stays in 8 bits: S = Q K^T as kind::f8f6f4 with Q in two e4m3 parts, q = hi + lo.  A bf16
 //     has 8 significant bits and each part holds 4: hi is the upper four, lo the rest.  After a
 //     power-of-two scaling of the row (maximum in [128, 256)) that is exact down to 2^-10 of the
@@ -148,7 +149,9 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
     uint8_t *sK = sQ + NS * 2 * C::KT;          // [KS]
     uint8_t *sR = sK + KS * C::KT;              // [RS] raw V
     uint8_t *sV = sR + RS * C::KT;              // [VS] f16 V, HD / 64 boxes of 128 rows x 128 bytes
-    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);  // [kEnt][8]: sk, log2 sv, sv0 / sv, (group 0) spread flag, (1) log2 sv0, (2) first token that is there
+    // [kEnt][8]: sk, log2 sv, sv0 / sv; then, in group 0, whether the scales are spread, in 1 log2 sv0, in 2 the first
+    // token that is there
+    float4 *ent = reinterpret_cast<float4 *>(sV + VS * C::VT);
     uint64_t *bars = reinterpret_cast<uint64_t *>(ent + kEnt * 8);
     uint64_t *k_full = bars;            // [KS]
     uint64_t *k_empty = k_full + KS;    // [KS] a commit per stream

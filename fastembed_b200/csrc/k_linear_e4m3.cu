@@ -15,7 +15,8 @@
 //   linear_e4m3_pair  a cluster pair computes a 256 x 256 tile (cta_group::2); calls of more than
 //                     a round of the SMs' tiles.
 //   linear_e4m3_cta   one CTA, 128 x BN tiles; few rows mean reading the weight, and that wants
-//                     every SM's loads in flight, so BN is the smallest that is one round of them.
+//                     many SMs' loads in flight, so BN is the smallest of 64, 128 and 256 that is one round
+//                     of them (at 64 columns 4,096 channels are 64 SMs).
 // K is never split: a row's result has the same bits in whatever batch, and so kernel, it comes.
 // Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (an elected lane), then the epilogue.
 // Every mbarrier wait is bounded; on timeout the CTA records FE_ERR_DEVICE_TIMEOUT in the device

@@ -361,7 +361,8 @@ fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int
  * max_kv_len is the caller's bound on past_lens[b] + len: it decides how sequences are split
  * over CTAs, not what is read.  Rows of out that belong to no sequence are left as they are; a
  * row that sees nothing (its pages are all out of range) is zero, one with a non-finite query
- * element that sees a token NaN, as is one whose logits pass fp32.  Scales may be any finite
+ * element that sees a token NaN, as is one whose logits (or scale times a page's key scale times the
+ * power of two of the query's largest element) pass fp32.  Scales may be any finite
  * positive numbers or 0; value codes of visible tokens must not be NaN (append writes none).
  * A query's elements are taken to 2^-16 of its largest (exact where they are above 2^-10 of it).
  * Weights are f16 relative to the row's largest (weights times value scales): 11 bits each, and
