@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(32 * WARPS) attn_cache_stream(const CacheArgs 
         }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        // 2^-e and 2^e of the row's exponent, e in [-100, 127]
+        // 2^-e and 2^e of the row's exponent, e in [-126, 127] (subnormal rows stay below 1, well above f16's steps)
         int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
-        e = e < -100 ? -100 : e;
+        e = e < -126 ? -126 : e;
         const float down = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
         const float up = __uint_as_float(static_cast<uint32_t>(127 + (e > 126 ? 126 : e)) << 23);
 #pragma unroll

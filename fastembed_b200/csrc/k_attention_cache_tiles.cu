@@ -460,7 +460,8 @@ __global__ void __launch_bounds__(TileCfg<HD>::THREADS, 1)
 #pragma unroll
                         for (int d = 1; d < LPR; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
                     }
-                    const int e = max(-100, static_cast<int>(m >> 7) - 127 - 7);  // q 2^-e has its maximum in [128, 256)
+                    // q 2^-e has its maximum in [128, 256); 2^e is a normal number, so in less below 2^-119
+                    const int e = max(-126, static_cast<int>(m >> 7) - 127 - 7);
                     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
                     // a negative softmax scale turns Q's signs, so that the logit factor is never negative
                     const float sign = a.scale_log2 < 0.f ? -down : down;

@@ -364,7 +364,8 @@ fe_status fe_attention_cache_workspace_bytes(int32_t batch, int32_t max_len, int
  * element that sees a token NaN, as is one whose logits (or scale times a page's key scale times the
  * power of two of the query's largest element) pass fp32.  Scales may be any finite
  * positive numbers or 0; value codes of visible tokens must not be NaN (append writes none).
- * A query's elements are taken to 2^-16 of its largest (exact where they are above 2^-10 of it).
+ * A query's elements are taken to 2^-16 of its largest (exact where they are above 2^-10 of it), or to
+ * 2^-135 where that is more.
  * Weights are f16 relative to the row's largest (weights times value scales): 11 bits each, and
  * 2^-32 of the largest at the least; sums are fp32.
  * max_len * q_heads / kv_heads is at most 65,535 * 128.

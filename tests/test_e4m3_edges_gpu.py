@@ -356,3 +356,36 @@ def test_offsets_that_run_backwards_are_reported(cuda_dev, new, bound):
     got = run(i32([0, a, a, a]), i32([40, -1, 50]))  # empty ones, whatever else stands there
     assert torch.equal(got[:a], want[:a]) and torch.all(got[a:] == 9.0)
     ops.device_status(0)
+
+
+# ------------------------------------------------------------ queries of any size
+@pytest.mark.parametrize("hd,heads", [(64, (4, 4)), (128, (4, 2)), (256, (3, 1))])
+@pytest.mark.parametrize("new,bound", [([3, 1], None), ([3, 1], 1 << 20), ([90, 40], None), ([200, 40], 1 << 20)])
+def test_queries_of_any_size(cuda_dev, hd, heads, new, bound):
+    """Queries from 1e-38 to 1e36 with a softmax scale that brings their logits back to ordinary size."""
+    from fastembed_b200 import ops
+    b = Batch(new, [150, 333], 32, *heads, hd, cuda_dev, seed=hd + 5)
+    cache = b.random_cache(ops)
+    ops.kv_cache_append_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, b.table, cache, b.q_heads)
+    x = b.qkv.view(sum(new), -1, hd)
+    q1 = x[:, :heads[0]].clone()
+    for size in (1e-38, 1e-36, 1e-34, 1e-30, 1e-25, 1.0, 1e20, 1e36):
+        x[:, :heads[0]] = (q1.double() * size).to(torch.bfloat16)
+        scale = hd ** -0.5 / size
+        if scale * math.log2(math.e) > 3.4e38:
+            x[:, :heads[0]], scale = x[:, :heads[0]] * 64, scale / 64
+        out = ops.attention_cache_e4m3(b.qkv, b.cu, b.max_new, b.past_lens, bound or b.max_kv, b.table, cache, heads[0], True, scale)
+        want, mag, dot, floor = ref.attention(cache, b.qkv, b.new, b.past, b.table, heads[0], True, scale)
+        # elements are off by 2^-16 of the row's largest, or 2^-135: times the largest sum of |k|, in numerator and
+        # denominator; the softmax scale in base 2 by two roundings
+        top = x[:, :heads[0]].abs().amax(-1).double()
+        kv = torch.cat([ref.values(cache.k.view(torch.uint8)[b.table[s, : -(-(n + p) // 32)].long()].view(F8),
+                                   cache.k_scale[b.table[s, : -(-(n + p) // 32)].long()]).abs().sum(-1).amax(-1)
+                        for s, (n, p) in enumerate(zip(b.new, b.past))]).amax(0)
+        off = torch.maximum(2.0 ** -16 * top, torch.tensor(2.0 ** -135, device=cuda_dev, dtype=torch.float64)) * abs(scale)
+        off = off * kv.repeat_interleave(heads[0] // heads[1])[None] + 2.0 ** -23 * dot.view(sum(new), heads[0], hd)[..., 0]
+        bound_ = ref.attention_bound(want, mag, dot, floor, hd) + (torch.expm1(2 * off)[..., None] * mag.view(-1, heads[0], hd)).reshape(
+            want.shape)
+        err = (out.double() - want).abs()
+        assert torch.all(err <= bound_), (size, float((err / bound_).max()))
+        ops.device_status(0)
