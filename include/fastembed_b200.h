@@ -314,7 +314,8 @@ fe_status fe_quantize_rows_e4m3(const void *x, fe_dtype x_dtype, int64_t rows, i
 /* h32 += y in place (y fp32 or bf16 [rows, dim]; NULL: no addition, h32 is not written), then
  * RMSNorm(h32) = h32 / sqrt(mean(h32^2) + eps) * w (1 + w when one_plus) as fe_quantize_rows_e4m3
  * of its rows.  Sum of squares and normalisation in fp32: a row whose sum of squares passes
- * 3.4e38 normalises to 0. */
+ * 3.4e38 normalises to 0, and with eps = 0 one whose squares vanish in fp32 is not finite (NaN
+ * codes). */
 fe_status fe_add_rmsnorm_e4m3(const void *y, fe_dtype y_dtype, float *h32, const float *w, int32_t one_plus, float eps,
                               int64_t rows, int32_t dim, void *q, float *scale, fe_stream_t stream);
 /* y[m,n] = epilogue(x_scale[i] * w_scale[j] * (x[m,k] . w[n,k]^T)) over e4m3 codes, one scale

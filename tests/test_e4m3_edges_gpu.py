@@ -127,6 +127,9 @@ def test_norm_of_a_row_whose_sum_of_squares_overflows(cuda_dev):
         q, s = ops.add_rmsnorm_e4m3(None, h, w, 1e-6)
         assert torch.all(q[1].float() == 0) and float(s[1]) == float(torch.tensor(2.0 ** -110) / torch.tensor(448.0))
         assert torch.all(q[0].float() == 448) and torch.all(q[2].float() == 448)
+        h[1] = 1e-30
+        q, s = ops.add_rmsnorm_e4m3(None, h, w, 0.0)  # without eps, squares that vanish leave nothing to divide by
+        assert torch.isnan(q[1].float()).all() and torch.all(q[0].float() == 448) and torch.all(q[2].float() == 448)
 
 
 # ------------------------------------------------------------ value scales of pages
